@@ -144,6 +144,44 @@ struct DenseFinalize {
   void *dw = nullptr, *db = nullptr, *dwh = nullptr, *dbh = nullptr;
 };
 
+// K22: embedding lookup out[i] = scale * W[id_i] (zeros for ids outside [0, V)) and its gradient
+// dW[v] = scale * sum of dy[i] over id_i = v, summed in fp32 in the order of i; `pad` (or -1) is a row whose
+// gradient stays zero. W rows are wstride elements apart, dy rows dystride; out and dW are dense. Element types are
+// the codes of vec_types.h. The workspace holds embedding_grad_workspace(n, V) bytes.
+void embedding_fwd(const void* ids, bool ids64, const void* w, int wtype, int64_t wstride, void* out, int otype,
+                   int64_t n, int64_t V, int64_t D, float scale, hipStream_t stream);
+int64_t embedding_grad_workspace(int64_t n, int64_t V);
+void embedding_grad(const void* ids, bool ids64, const void* dy, int otype, int64_t dystride, void* dw, int wtype,
+                    int64_t n, int64_t V, int64_t D, int64_t pad, float scale, void* workspace, hipStream_t stream);
+
+// K23: out = residual + dropout(x) over n consecutive elements (residual may be null). The counter of the generator is
+// `offset`, or *ctr where ctr is given; `used` (may be null) receives it, for a backward pass with the same mask.
+void dropout(const void* x, const void* res, void* out, int type, int64_t n, double p, uint64_t seed, uint64_t offset,
+             const int64_t* ctr, int64_t* used, hipStream_t stream);
+
+// K24: gated linear recurrence h_t = (1 - z_t) h_{t-1} + z_t x_t, z = sigmoid(g), over [B, L, D]. Strides are in
+// elements for sequence (sb) and step (st); channels are consecutive. y is dense.
+struct ScanArgs {
+  int64_t B = 0, L = 0, D = 0;
+  int64_t xsb = 0, xst = 0, gsb = 0, gst = 0;  // x and g
+  int64_t ysb = 0, yst = 0;                    // dy
+  int64_t dsb = 0, dst = 0;                    // dx and dg (one layout for both)
+  const float* h0 = nullptr;                   // [B, D], null: zeros
+  const uint8_t* resets = nullptr;             // [B, L], null: none
+  const int64_t* lengths = nullptr;            // [B], null: all L
+  float* ckpt = nullptr;                       // [B, gated_scan_checkpoints(L), D]: written by fwd (null: not), read by bwd
+  float* h_last = nullptr;                     // [B, D]
+  const float* dh_last = nullptr;              // [B, D], null: zeros
+  float* dh0 = nullptr;                        // [B, D], null: not wanted
+};
+int64_t gated_scan_checkpoints(int64_t L);
+void gated_scan_fwd(const ScanArgs& p, const void* x, const void* g, void* y, int type, hipStream_t stream);
+void gated_scan_bwd(const ScanArgs& p, const void* x, const void* g, const void* dy, void* dx, void* dg, int type,
+                    hipStream_t stream);
+// one step of B sequences: out (may be h itself) = the new states [B, D], y = the same in the element type
+void gated_scan_step(const void* x, int64_t xs, const void* g, int64_t gs, const uint8_t* resets, const float* h,
+                     float* out, void* y, int type, int64_t B, int64_t D, hipStream_t stream);
+
 // K11: shuffle partitioning. dest = splitmix64(key) % R (mode 0) or key mod R (mode 1), R <= 1024.
 // partition_hist writes counts[G][R] (G = partition_groups(n)); the caller turns them into
 // exclusive offsets (destination-major: all of destination 0's rows first) and partition_scatter

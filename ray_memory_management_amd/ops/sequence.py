@@ -1,0 +1,461 @@
+"""Operators of token and sequence models: embedding with a sorted gradient, counter-based dropout and the gated
+linear recurrence (kernels K22-K24 in ``csrc/hip/{embedding,dropout,scan}_kernels.hip``).
+
+CUDA(ROCm) tensors run the HIP kernels on the current stream of their device; CPU tensors the same formulas in torch.
+fp32, bf16 and fp16 are taken on the GPU; sums and states are held in fp32. Everything here can be captured into a
+graph: nothing synchronises, and what a call keeps for its backward pass belongs to that call.
+"""
+from __future__ import annotations
+
+import contextlib
+from typing import Optional, Tuple, Union
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from ray_memory_management_amd._native import require_hip
+
+__all__ = ["embedding", "Embedding", "dropout", "Dropout", "gated_scan", "gated_scan_step"]
+
+_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # vec_types.h ElemType
+_NULL = contextlib.nullcontext()
+
+
+def _stream(t: torch.Tensor) -> int:
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _device(t: torch.Tensor):
+    """Context in which t's device is the current one (launches go to the current device)."""
+    return _NULL if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _code(who: str, t: torch.dtype) -> int:
+    c = _CODE.get(t)
+    if c is None:
+        raise ValueError(f"{who}: fp32, bf16 or fp16 tensors on the GPU, not {t}")
+    return c
+
+
+def _same_device(who: str, ref: torch.Tensor, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != ref.device:
+            raise ValueError(f"{who}: {name} is on {t.device}, not on {ref.device}")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t with consecutive elements in its last dimension."""
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+# ------------------------------------------------------------------------------------------ embedding
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding_idx, dtype):
+        h = require_hip()
+        V, D = weight.shape
+        n = ids.numel()
+        w = _rows(weight.detach())
+        out = torch.empty((*ids.shape, D), dtype=dtype, device=weight.device)
+        with _device(weight):
+            h.embedding_fwd(ids.data_ptr(), ids.dtype == torch.int64, w.data_ptr(), _CODE[w.dtype], w.stride(0),
+                            out.data_ptr(), _CODE[dtype], n, V, D, scale, _stream(weight))
+        ctx.save_for_backward(ids)
+        ctx.meta = (V, D, scale, padding_idx, weight.dtype)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (ids,) = ctx.saved_tensors
+        V, D, scale, padding_idx, dtype = ctx.meta
+        h = require_hip()
+        n = ids.numel()
+        dy = _rows(dy.reshape(n, D))
+        dw = torch.empty((V, D), dtype=dtype, device=dy.device)
+        ws = torch.empty(h.embedding_grad_workspace(n, V), dtype=torch.uint8, device=dy.device)
+        with _device(dy):
+            h.embedding_grad(ids.data_ptr(), ids.dtype == torch.int64, dy.data_ptr(), _CODE[dy.dtype], dy.stride(0),
+                             dw.data_ptr(), _CODE[dtype], n, V, D, padding_idx, scale, ws.data_ptr(), _stream(dy))
+        return None, dw, None, None, None
+
+
+def _embedding_cpu(ids, weight, scale, padding_idx, dtype):
+    ids = ids.long()
+    ok = (ids >= 0) & (ids < weight.shape[0])
+    w = weight if weight.dtype in (torch.float32, torch.float64) else weight.float()
+    pad = padding_idx if padding_idx >= 0 else None
+    if bool(ok.all()):
+        out = nn.functional.embedding(ids, w, pad)
+    elif weight.shape[0] == 0:
+        out = w.new_zeros((*ids.shape, w.shape[1]))
+    else:
+        out = nn.functional.embedding(torch.where(ok, ids, torch.zeros_like(ids)), w, pad)
+        out = torch.where(ok.unsqueeze(-1), out, torch.zeros((), dtype=out.dtype))
+    return (out if scale == 1.0 else out * scale).to(dtype)
+
+
+def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None,
+              dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``out[...] = scale * weight[ids[...]]``, rounded once to ``dtype`` (weight's type by default).
+
+    ids: int32 / int64 of any shape; an id outside ``[0, len(weight))`` gives a row of zeros and no gradient, so -1
+    can mark padded places. weight: [V, D]. Its gradient is dense, ``scale * sum of dy over the places of an id``,
+    summed in fp32 in the order of the places (the same bits every time) and rounded once; the row ``padding_idx``
+    (negative counts from the end) is read as any other and gets no gradient."""
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"embedding: int32 or int64 ids, not {ids.dtype}")
+    if weight.dim() != 2:
+        raise ValueError(f"embedding: weight must be [V, D], not {tuple(weight.shape)}")
+    _same_device("embedding", weight, ids=ids)
+    V, pad, dtype = weight.shape[0], -1, dtype or weight.dtype
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
+            raise ValueError(f"embedding: padding_idx {padding_idx} outside the {V} rows")
+        pad = int(padding_idx) % V
+    if not dtype.is_floating_point or not weight.dtype.is_floating_point:
+        raise ValueError("embedding: floating-point weight and output types")
+    if weight.device.type != "cuda":
+        return _embedding_cpu(ids, weight, float(scale), pad, dtype)
+    _code("embedding", weight.dtype), _code("embedding", dtype)
+    if max(ids.numel(), V) >= 2 ** 31 - 1:
+        raise ValueError("embedding: fewer than 2^31 - 1 ids and rows")
+    return _Embedding.apply(ids.contiguous(), weight, float(scale), pad, dtype)
+
+
+class Embedding(nn.Embedding):
+    """``nn.Embedding`` through :func:`embedding`: the same parameters and state dict, with a ``scale`` on the output.
+    ``max_norm``, ``scale_grad_by_freq`` and ``sparse`` are not supported."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, padding_idx: Optional[int] = None, scale: float = 1.0,
+                 **kw):
+        for k in ("max_norm", "scale_grad_by_freq", "sparse"):
+            if kw.get(k):
+                raise ValueError(f"Embedding: {k} is not supported")
+        super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, **kw)
+        self.scale = float(scale)
+
+    def forward(self, ids):
+        return embedding(ids, self.weight, self.scale, self.padding_idx)
+
+
+# ------------------------------------------------------------------------------------------ dropout
+_M32 = 0xFFFFFFFF
+
+
+def _mulhilo(m: int, x: torch.Tensor):
+    """High and low word of m * x for 32-bit words held in int64 (the product itself could pass 63 bits)."""
+    low, high = (m & 0xFFFF) * x, (m >> 16) * x
+    mid = (low >> 16) + high
+    return mid >> 16, ((mid & 0xFFFF) << 16) | (low & 0xFFFF)
+
+
+def _philox_words(index: torch.Tensor, offset: int, seed: int) -> torch.Tensor:
+    """The four 32-bit words (int64, [n, 4]) of Philox4x32-10 (Salmon et al. 2011) at counter (index, offset)."""
+    a, b = index & _M32, (index >> 32) & _M32
+    c, d = torch.full_like(index, offset & _M32), torch.full_like(index, (offset >> 32) & _M32)
+    k0, k1 = seed & _M32, (seed >> 32) & _M32
+    for _ in range(10):
+        h0, l0 = _mulhilo(0xD2511F53, a)
+        h1, l1 = _mulhilo(0xCD9E8D57, c)
+        a, b, c, d = h1 ^ b ^ k0, l1, h0 ^ d ^ k1, l0
+        k0, k1 = (k0 + 0x9E3779B9) & _M32, (k1 + 0xBB67AE85) & _M32
+    return torch.stack([a, b, c, d], dim=-1)
+
+
+def _threshold(p: float) -> int:
+    return int(round(p * 65536))
+
+
+def _dropout_cpu(x, p, seed, offset, residual):
+    n, t = x.numel(), _threshold(p)
+    w = _philox_words(torch.arange((n + 7) // 8), int(offset), seed)
+    keep = torch.stack([w & 0xFFFF, w >> 16], dim=-1).reshape(-1)[:n].reshape(x.shape) >= t
+    acc = x if x.dtype == torch.float64 else x.float()
+    # the dropped places go out before the product, so that what they hold reaches neither result nor gradient
+    y = torch.where(keep, acc, torch.zeros((), dtype=acc.dtype)) * (65536.0 / (65536 - t) if t < 65536 else 0.0)
+    return (y if residual is None else y + residual.to(y.dtype)).to(x.dtype)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, offset):
+        xc = x.detach().contiguous()
+        rc = None if residual is None else residual.detach().contiguous()
+        out = torch.empty_like(xc)
+        ctr = offset if isinstance(offset, torch.Tensor) else None
+        used = torch.empty(1, dtype=torch.int64, device=x.device) if ctr is not None else None
+        with _device(x):
+            require_hip().dropout(xc.data_ptr(), _ptr(rc), out.data_ptr(), _CODE[x.dtype], xc.numel(), p, seed,
+                                  0 if ctr is not None else offset, _ptr(ctr), _ptr(used), _stream(x))
+        ctx.save_for_backward(used)
+        ctx.meta = (p, seed, 0 if ctr is not None else offset)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (used,) = ctx.saved_tensors
+        p, seed, offset = ctx.meta
+        dx = None
+        if ctx.needs_input_grad[0]:
+            d = dy.contiguous()
+            dx = torch.empty_like(d)
+            with _device(d):
+                require_hip().dropout(d.data_ptr(), 0, dx.data_ptr(), _CODE[d.dtype], d.numel(), p, seed, offset,
+                                      _ptr(used), 0, _stream(d))
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+
+
+def dropout(x: torch.Tensor, p: float, seed: int, offset: Union[int, torch.Tensor] = 0,
+            residual: Optional[torch.Tensor] = None, training: bool = True) -> torch.Tensor:
+    """``residual + dropout(x)`` whose mask is a function of (seed, offset, element index) and never stored.
+
+    An element is dropped (zero, whatever it held) where its 16 random bits are below ``t = round(65536 p)``, else
+    scaled by ``65536 / (65536 - t)``; the bits are those of Philox4x32-10 with key ``seed`` and counter
+    (index // 8, offset), so the CPU and the GPU draw the same mask. Elements are numbered in row-major order.
+
+    offset: the call's own number under the seed: an int, or an int64 tensor on x's device whose first element is read
+    when the kernel runs (a graph replay then draws a new mask after each advance); the backward pass uses the value
+    that its forward pass read. residual: same shape and type as x."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout: p must be in [0, 1], not {p}")
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError(f"dropout: residual must match x: {tuple(residual.shape)} {residual.dtype} against "
+                             f"{tuple(x.shape)} {x.dtype}")
+    if isinstance(offset, torch.Tensor):
+        if offset.dtype != torch.int64 or offset.numel() < 1:
+            raise ValueError("dropout: an offset tensor holds int64")
+        _same_device("dropout", x, offset=offset)
+    else:
+        offset = int(offset) & 0xFFFFFFFFFFFFFFFF
+    _same_device("dropout", x, residual=residual)
+    if not x.dtype.is_floating_point:
+        raise ValueError(f"dropout: a floating-point tensor, not {x.dtype}")
+    if not training:
+        return x if residual is None else x + residual
+    seed = int(seed) & 0xFFFFFFFFFFFFFFFF
+    if x.device.type != "cuda":
+        if isinstance(offset, torch.Tensor):
+            offset = int(offset.reshape(-1)[0])
+        return _dropout_cpu(x, float(p), seed, offset, residual)
+    _code("dropout", x.dtype)
+    return _Dropout.apply(x, residual, float(p), seed, offset)
+
+
+class Dropout(nn.Module):
+    """Dropout layer over :func:`dropout`. Its call counter is a buffer on the layer's device that every training call
+    advances there, so a captured graph draws a new mask on each replay and a restored state dict goes on where it was
+    saved. Layers of one model take different seeds."""
+
+    def __init__(self, p: float = 0.5, seed: int = 0):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"Dropout: p must be in [0, 1], not {p}")
+        self.p, self.seed = float(p), int(seed)
+        self.register_buffer("counter", torch.zeros(1, dtype=torch.int64))
+
+    def forward(self, x, residual=None):
+        if not self.training or self.p == 0.0:
+            return dropout(x, self.p, self.seed, residual=residual, training=False)
+        y = dropout(x, self.p, self.seed, self.counter, residual)
+        self.counter.add_(1)
+        return y
+
+    def extra_repr(self):
+        return f"p={self.p}, seed={self.seed}"
+
+
+# ------------------------------------------------------------------------------------------ gated scan
+class _Gate(torch.autograd.Function):
+    """sigmoid(g) and 1 - sigmoid(g) with their relative precision on both sides, in the gradient too (that of
+    torch.sigmoid takes 1 - z by a subtraction, which has none left near z = 1)."""
+
+    @staticmethod
+    def forward(ctx, g):
+        z, a = torch.sigmoid(g), torch.sigmoid(-g)
+        ctx.save_for_backward(z, a)
+        return z, a
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dz, da):
+        z, a = ctx.saved_tensors
+        return (dz - da) * z * a
+
+
+def _scan_cpu(x, gate, h0, resets, lengths):
+    B, L, D = x.shape
+    ct = torch.promote_types(x.dtype, torch.float32)
+    st = torch.promote_types(ct, h0.dtype)
+    x, gate, h, zero = x.to(ct), gate.to(ct), h0.to(st), torch.zeros((), dtype=ct)
+    live = None
+    if lengths is not None:
+        live = (torch.arange(L) < lengths.unsqueeze(1)).unsqueeze(-1)
+        x, gate = torch.where(live, x, zero), torch.where(live, gate, zero)
+    z, a = _Gate.apply(gate)
+    ys = []
+    for t in range(L):
+        prev = h if resets is None else torch.where(resets[:, t, None], torch.zeros((), dtype=st), h)
+        new = a[:, t] * prev + z[:, t] * x[:, t]
+        h = new if live is None else torch.where(live[:, t], new, h)
+        ys.append(new if live is None else torch.where(live[:, t], new, torch.zeros((), dtype=new.dtype)))
+    return (torch.stack(ys, dim=1) if L else x.new_zeros((B, 0, D), dtype=st)), h
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, h0, resets, lengths):
+        ctx.set_materialize_grads(False)
+        h = require_hip()
+        x = _rows(x.detach())
+        B, L, D = x.shape
+        if gate is None:
+            D //= 2
+            g, gs, gp = None, (x.stride(0), x.stride(1)), x.data_ptr() + D * x.element_size()
+        else:
+            g = _rows(gate.detach())
+            gs, gp = (g.stride(0), g.stride(1)), g.data_ptr()
+        y = torch.empty((B, L, D), dtype=x.dtype, device=x.device)
+        h_last = torch.empty((B, D), dtype=torch.float32, device=x.device)
+        ckpt = None
+        if any(ctx.needs_input_grad):
+            ckpt = torch.empty((B, h.gated_scan_checkpoints(L), D), dtype=torch.float32, device=x.device)
+        with _device(x):
+            h.gated_scan_fwd(x.data_ptr(), gp, y.data_ptr(), _CODE[x.dtype], (B, L, D),
+                             (x.stride(0), x.stride(1), *gs), _ptr(h0), _ptr(resets), _ptr(lengths), _ptr(ckpt),
+                             h_last.data_ptr(), _stream(x))
+        ctx.save_for_backward(x, g, resets, lengths, ckpt)
+        return y, h_last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh):
+        x, g, resets, lengths, ckpt = ctx.saved_tensors
+        h = require_hip()
+        B, L, D = x.shape
+        if g is None:
+            D //= 2
+            gs, gp = (x.stride(0), x.stride(1)), x.data_ptr() + D * x.element_size()
+            dx, dg, ds = torch.empty((B, L, 2 * D), dtype=x.dtype, device=x.device), None, (L * 2 * D, 2 * D)
+            dgp = dx.data_ptr() + D * x.element_size()
+        else:
+            gs, gp = (g.stride(0), g.stride(1)), g.data_ptr()
+            dx, dg = (torch.empty((B, L, D), dtype=x.dtype, device=x.device) for _ in range(2))
+            ds, dgp = (L * D, D), dg.data_ptr()
+        dh0 = torch.empty((B, D), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
+        dy = None if dy is None else _rows(dy)
+        dh = None if dh is None else dh.contiguous()
+        ys = (0, 0) if dy is None else (dy.stride(0), dy.stride(1))
+        with _device(x):
+            h.gated_scan_bwd(x.data_ptr(), gp, _ptr(dy), dx.data_ptr(), dgp, _CODE[x.dtype], (B, L, D),
+                             (x.stride(0), x.stride(1), *gs, *ys, *ds), _ptr(resets), _ptr(lengths), _ptr(ckpt),
+                             _ptr(dh), _ptr(dh0), _stream(x))
+        return dx, dg, dh0, None, None
+
+
+def _scan_parts(who, x, gate):
+    """Checks x and gate; the channel count."""
+    if x.dim() != (3 if who == "gated_scan" else 2):
+        raise ValueError(f"{who}: x must be {'[B, L, D]' if who == 'gated_scan' else '[B, D]'}, not {tuple(x.shape)}")
+    if not x.dtype.is_floating_point:
+        raise ValueError(f"{who}: a floating-point tensor, not {x.dtype}")
+    if gate is None:
+        if x.shape[-1] % 2:
+            raise ValueError(f"{who}: without a gate, x holds the inputs and the gates in halves of one size; "
+                             f"{x.shape[-1]} channels")
+        return x.shape[-1] // 2
+    if gate.shape != x.shape or gate.dtype != x.dtype:
+        raise ValueError(f"{who}: gate must match x: {tuple(gate.shape)} {gate.dtype} against {tuple(x.shape)} {x.dtype}")
+    return x.shape[-1]
+
+
+def _flags(who, resets, shape):
+    if resets is None:
+        return None
+    if tuple(resets.shape) != tuple(shape):
+        raise ValueError(f"{who}: resets must be {tuple(shape)}, not {tuple(resets.shape)}")
+    resets = resets if resets.dtype == torch.bool else resets != 0
+    return resets.contiguous()
+
+
+def gated_scan(x: torch.Tensor, gate: Optional[torch.Tensor] = None, h0: Optional[torch.Tensor] = None,
+               resets: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None
+               ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Gated linear recurrence over [B, L, D]: ``h_t = (1 - z_t) h_{t-1} + z_t x_t`` with ``z = sigmoid(gate)``.
+
+    Returns (y, h_last): y [B, L, D] the states in x's type, h_last [B, D] the fp32 state behind the last step.
+    Differentiable in x, gate and h0.
+
+    x, gate: same shape and type; any strides with consecutive channels are read in place. Without ``gate``, x is
+    [B, L, 2D], inputs and gates in its halves as one projection gives them, and so is its gradient.
+    h0: [B, D] state before the first step (zeros by default). resets: [B, L], non-zero where the state is dropped
+    before the step (an episode or document begins). lengths: [B] integers, steps of each sequence (clamped to
+    [0, L]): later places take no part whatever they hold, their y and gradients are 0."""
+    D = _scan_parts("gated_scan", x, gate)
+    B, L = x.shape[:2]
+    _same_device("gated_scan", x, gate=gate, h0=h0, resets=resets, lengths=lengths)
+    if h0 is not None and tuple(h0.shape) != (B, D):
+        raise ValueError(f"gated_scan: h0 must be {(B, D)}, not {tuple(h0.shape)}")
+    if lengths is not None and (tuple(lengths.shape) != (B,) or lengths.dtype.is_floating_point
+                                or lengths.dtype.is_complex or lengths.dtype == torch.bool):
+        raise ValueError(f"gated_scan: lengths must be {B} integers, not {tuple(lengths.shape)} {lengths.dtype}")
+    resets = _flags("gated_scan", resets, (B, L))
+    if x.device.type != "cuda":
+        if gate is None:
+            x, gate = x[..., :D], x[..., D:]
+        h0 = x.new_zeros((B, D), dtype=torch.promote_types(x.dtype, torch.float32)) if h0 is None else h0
+        y, h = _scan_cpu(x, gate, h0, resets, lengths)
+        return y.to(x.dtype), h.to(torch.promote_types(x.dtype, torch.float32))
+    _code("gated_scan", x.dtype)
+    h0 = None if h0 is None else h0.to(torch.float32).contiguous()
+    lengths = None if lengths is None else lengths.to(torch.int64).contiguous()
+    return _GatedScan.apply(x, gate, h0, None if resets is None else resets.view(torch.uint8), lengths)
+
+
+def gated_scan_step(x: torch.Tensor, gate: Optional[torch.Tensor], state: torch.Tensor,
+                    resets: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None
+                    ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """One step of :func:`gated_scan` for B running sequences: returns (y [B, D] in x's type, new state [B, D] fp32).
+
+    x, gate: [B, D] (or x [B, 2D] and gate None). state: [B, D] fp32, consecutive. resets: [B]. out: where the new state
+    goes; ``out=state`` updates it in place. Not differentiable: with gradients, call :func:`gated_scan` with L = 1."""
+    D = _scan_parts("gated_scan_step", x, gate)
+    B = x.shape[0]
+    _same_device("gated_scan_step", x, gate=gate, state=state, resets=resets, out=out)
+    for name, t in (("state", state), ("out", out)):
+        if t is not None and (tuple(t.shape) != (B, D) or t.dtype != torch.float32 or not t.is_contiguous()):
+            raise ValueError(f"gated_scan_step: {name} must be {(B, D)}, fp32 and contiguous")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, state)):
+        raise ValueError("gated_scan_step is not differentiable: call gated_scan with L = 1, or under torch.no_grad()")
+    if out is not None:
+        delta = abs(out.data_ptr() - state.data_ptr())
+        if 0 < delta < state.numel() * 4:
+            raise ValueError("gated_scan_step: out overlaps state without being it")
+    resets = _flags("gated_scan_step", resets, (B,))
+    if x.device.type != "cuda":
+        if gate is None:
+            x, gate = x[..., :D], x[..., D:]
+        prev = state if resets is None else torch.where(resets.unsqueeze(-1), torch.zeros(()), state)
+        h = torch.sigmoid(-gate.float()) * prev + torch.sigmoid(gate.float()) * x.float()
+        out = h if out is None else out.copy_(h)
+        return out.to(x.dtype, copy=True), out
+    code = _code("gated_scan_step", x.dtype)
+    x = _rows(x)
+    if gate is None:
+        gp, gs = x.data_ptr() + D * x.element_size(), x.stride(0)
+    else:
+        gate = _rows(gate)
+        gp, gs = gate.data_ptr(), gate.stride(0)
+    out = torch.empty_like(state) if out is None else out
+    y = torch.empty((B, D), dtype=x.dtype, device=x.device)
+    with _device(x):
+        require_hip().gated_scan_step(x.data_ptr(), x.stride(0), gp, gs, _ptr(resets), state.data_ptr(),
+                                      out.data_ptr(), y.data_ptr(), code, B, D, _stream(x))
+    return y, out

@@ -314,26 +314,28 @@ PYBIND11_MODULE(_hip, m) {
             P<int64_t>(used), S(stream));
   });
   m.def("gated_scan_checkpoints", &gated_scan_checkpoints);
+  m.def("gated_scan_workspace", &gated_scan_workspace);
   // dims = B, L, D; strides = x (sequence, step), gate, [dy, gradients]
   m.def("gated_scan_fwd", [](uint64_t x, uint64_t g, uint64_t y, int type, std::array<int64_t, 3> dims,
                              std::array<int64_t, 4> st, uint64_t h0, uint64_t resets, uint64_t lengths, uint64_t ckpt,
-                             uint64_t h_last, uint64_t stream) {
+                             uint64_t h_last, uint64_t ws, uint64_t stream) {
     ScanArgs p;
     p.B = dims[0], p.L = dims[1], p.D = dims[2];
     p.xsb = st[0], p.xst = st[1], p.gsb = st[2], p.gst = st[3];
     p.h0 = P<const float>(h0), p.resets = P<const uint8_t>(resets), p.lengths = P<const int64_t>(lengths);
-    p.ckpt = P<float>(ckpt), p.h_last = P<float>(h_last);
+    p.ckpt = P<float>(ckpt), p.h_last = P<float>(h_last), p.workspace = P<void>(ws);
     gated_scan_fwd(p, P<const void>(x), P<const void>(g), P<void>(y), type, S(stream));
   });
   m.def("gated_scan_bwd", [](uint64_t x, uint64_t g, uint64_t dy, uint64_t dx, uint64_t dg, int type,
                              std::array<int64_t, 3> dims, std::array<int64_t, 8> st, uint64_t resets, uint64_t lengths,
-                             uint64_t ckpt, uint64_t dh_last, uint64_t dh0, uint64_t stream) {
+                             uint64_t ckpt, uint64_t dh_last, uint64_t dh0, uint64_t ws, uint64_t stream) {
     ScanArgs p;
     p.B = dims[0], p.L = dims[1], p.D = dims[2];
     p.xsb = st[0], p.xst = st[1], p.gsb = st[2], p.gst = st[3];
     p.ysb = st[4], p.yst = st[5], p.dsb = st[6], p.dst = st[7];
     p.resets = P<const uint8_t>(resets), p.lengths = P<const int64_t>(lengths);
     p.ckpt = P<float>(ckpt), p.dh_last = P<const float>(dh_last), p.dh0 = P<float>(dh0);
+    p.workspace = P<void>(ws);
     gated_scan_bwd(p, P<const void>(x), P<const void>(g), P<const void>(dy), P<void>(dx), P<void>(dg), type, S(stream));
   });
   m.def("gated_scan_step", [](uint64_t x, int64_t xs, uint64_t g, int64_t gs, uint64_t resets, uint64_t h, uint64_t out,

@@ -169,12 +169,14 @@ struct ScanArgs {
   const float* h0 = nullptr;                   // [B, D], null: zeros
   const uint8_t* resets = nullptr;             // [B, L], null: none
   const int64_t* lengths = nullptr;            // [B], null: all L
-  float* ckpt = nullptr;                       // [B, gated_scan_checkpoints(L), D]: written by fwd (null: not), read by bwd
+  float* ckpt = nullptr;                       // [B, gated_scan_checkpoints(L, type), D]: written by fwd (null: not), read by bwd
+  void* workspace = nullptr;                   // gated_scan_workspace(B, L, D, type) bytes, 8-byte aligned
   float* h_last = nullptr;                     // [B, D]
   const float* dh_last = nullptr;              // [B, D], null: zeros
   float* dh0 = nullptr;                        // [B, D], null: not wanted
 };
-int64_t gated_scan_checkpoints(int64_t L);
+int64_t gated_scan_checkpoints(int64_t L, int type);
+int64_t gated_scan_workspace(int64_t B, int64_t L, int64_t D, int type);
 void gated_scan_fwd(const ScanArgs& p, const void* x, const void* g, void* y, int type, hipStream_t stream);
 void gated_scan_bwd(const ScanArgs& p, const void* x, const void* g, const void* dy, void* dx, void* dg, int type,
                     hipStream_t stream);

@@ -8,10 +8,23 @@
 //   dh_t = dy_t + (1 - z_{t+1}) dh_{t+1}  (0 across a reset),    dx_t = z_t dh_t,
 //   dg_t = dh_t (x_t - h_{t-1}) z_t (1 - z_t),                   dh0  = (1 - z_0) dh_0
 //
-// The forward pass leaves the fp32 state at every kTS-th step, from which the backward pass recomputes h_{t-1}:
-// that reads less than a stored h would and keeps the rounding of y out of the gradient.
+// The forward pass leaves the fp32 state at the start of every chunk of K steps (K = 16, for fp32 tensors 8), from
+// which the backward pass recomputes h_{t-1}: that reads less than a stored h would (4 / K bytes an element against the
+// element itself) and keeps the rounding of y out of the gradient.
 //
-// One lane per (sequence, channel); the loads of kTS steps are issued together.
+// Split. Either pass is a composition of affine maps s -> A s + H, one per step. A wave takes a chunk of K steps of
+// 64 VEC channels, loads it whole into registers (every load in flight at once) and composes its K maps per lane; the
+// 1 to 4 waves of a workgroup, consecutive chunks, exchange their compositions through LDS; and where a sequence is
+// longer than that, workgroups pass the state on in one launch: each publishes its composition as soon as it has it,
+// looks back over its predecessors' until it meets a finished state, publishes its own finished state, and writes its
+// rows. So x, g (and dy) cross the memory bus once for any L, and few channels still fill the card.
+//
+// Waiting. A published word is one 64-bit atomic (A, H) that carries its own readiness in A: all ones before it is
+// written, -1 for a finished state, else in [0, 1]. Workgroups take their place from a ticket counter, and wait only for
+// lower tickets, whose workgroups therefore run already: by induction over the tickets every wait ends.
+//
+// A = 0 stands for a reset alone: what is before it is dropped, not multiplied by zero (it may be infinite or NaN).
+// Products that underflow are held at the smallest denormal instead, so an infinite state stays infinite.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -26,7 +39,14 @@ namespace hip {
 
 namespace {
 
-constexpr int kTS = 16;  // steps between saved states
+constexpr int kScanWaves = 4;  // most waves of a workgroup
+constexpr float kTiny = 1.4e-45f;
+constexpr uint32_t kFinished = 0xBF800000u;  // -1.0f in the place of A
+
+template <typename T>
+constexpr int chunk_steps() {
+  return sizeof(T) == 4 ? 8 : 16;
+}
 
 // z = sigmoid(g) and a = 1 - z, both to full relative precision: from exp(-|g|), which cannot overflow.
 __device__ __forceinline__ void gate_of(float g, float& z, float& a) {
@@ -42,85 +62,298 @@ __device__ __forceinline__ int64_t length_of(const int64_t* __restrict__ lengths
   return n < 0 ? 0 : n > L ? L : n;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kWave) void k_scan_fwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
-                                                    T* __restrict__ y) {
-  const int64_t d = int64_t(blockIdx.x) * kWave + threadIdx.x, b = blockIdx.y;
-  if (d >= p.D) return;
-  const int64_t n = length_of(p.lengths, b, p.L), nck = (p.L + kTS - 1) / kTS;
-  const T *xp = x + b * p.xsb + d, *gp = g + b * p.gsb + d;
-  const uint8_t* rp = p.resets ? p.resets + b * p.L : nullptr;
-  float h = p.h0 ? p.h0[b * p.D + d] : 0.f;
-  for (int64_t t0 = 0; t0 < p.L; t0 += kTS) {
-    if (p.ckpt) p.ckpt[(b * nck + t0 / kTS) * p.D + d] = h;
-    float xv[kTS], gv[kTS];
-#pragma unroll
-    for (int i = 0; i < kTS; i++) {
-      if (t0 + i < n) {
-        xv[i] = to_f32(xp[(t0 + i) * p.xst]);
-        gv[i] = to_f32(gp[(t0 + i) * p.gst]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kTS; i++) {
-      if (t0 + i < n) {
-        float z, a;
-        gate_of(gv[i], z, a);
-        h = rp && rp[t0 + i] ? z * xv[i] : fmaf(a, h, z * xv[i]);
-      }
-      if (t0 + i < p.L) y[(b * p.L + t0 + i) * p.D + d] = from_f32<T>(t0 + i < n ? h : 0.f);
-    }
-  }
-  p.h_last[b * p.D + d] = h;
+struct Map {  // s -> A s + H, A = 0: s is dropped
+  float A, H;
+};
+
+__device__ __forceinline__ float apply(const Map& m, float s) { return m.A == 0.f ? m.H : fmaf(m.A, s, m.H); }
+
+// `later` after `first`
+__device__ __forceinline__ Map then(const Map& first, const Map& later) {
+  if (later.A == 0.f) return later;
+  return Map{first.A == 0.f ? 0.f : fmaxf(first.A * later.A, kTiny), fmaf(later.A, first.H, later.H)};
 }
 
-template <typename T>
-__global__ __launch_bounds__(kWave) void k_scan_bwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
-                                                    const T* __restrict__ dy, T* __restrict__ dx, T* __restrict__ dg) {
-  const int64_t d = int64_t(blockIdx.x) * kWave + threadIdx.x, b = blockIdx.y;
-  if (d >= p.D) return;
-  const int64_t n = length_of(p.lengths, b, p.L), nck = (p.L + kTS - 1) / kTS;
-  const T *xp = x + b * p.xsb + d, *gp = g + b * p.gsb + d, *yp = dy ? dy + b * p.ysb + d : nullptr;
-  const uint8_t* rp = p.resets ? p.resets + b * p.L : nullptr;
-  float dh = p.dh_last ? p.dh_last[b * p.D + d] : 0.f;  // gradient reaching the state behind the step at hand
-  for (int64_t k = nck - 1; k >= 0; k--) {
-    const int64_t t0 = k * kTS;
-    float h = p.ckpt[(b * nck + k) * p.D + d];
-    float xv[kTS], gv[kTS], yv[kTS], hp[kTS];
+__device__ __forceinline__ uint64_t pack(float a, float h) {
+  return (uint64_t(__float_as_uint(a)) << 32) | __float_as_uint(h);
+}
+
+__device__ __forceinline__ uint64_t peek(const uint64_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ void publish(uint64_t* p, uint64_t v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__global__ __launch_bounds__(256) void k_scan_init(uint64_t* __restrict__ words, int64_t n, uint32_t* __restrict__ ticket) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) words[i] = ~0ull;
+}
+
+// States that reach segment `seg` (> 0) of VEC neighbouring chains whose words lie `stride` apart. kLook words of each are
+// read at a time: they do not depend on each other, so a walk over many unfinished predecessors costs one latency per
+// kLook.
+constexpr int kLook = 8;
+template <int VEC>
+__device__ __forceinline__ void look_back(const uint64_t* __restrict__ word, int64_t seg, int64_t stride,
+                                          float (&out)[VEC]) {
+  Map acc[VEC];
+  bool done[VEC], all = false;
 #pragma unroll
-    for (int i = 0; i < kTS; i++) {
-      if (t0 + i < n) {
-        xv[i] = to_f32(xp[(t0 + i) * p.xst]);
-        gv[i] = to_f32(gp[(t0 + i) * p.gst]);
-        yv[i] = yp ? to_f32(yp[(t0 + i) * p.yst]) : 0.f;
-      }
-    }
+  for (int v = 0; v < VEC; v++) acc[v] = Map{1.f, 0.f}, done[v] = false;
+  for (int64_t j = seg - 1; j >= 0 && !all; j -= kLook) {
+    uint64_t w[kLook][VEC];
 #pragma unroll
-    for (int i = 0; i < kTS; i++) {
-      if (t0 + i < n) {
-        float z, a;
-        gate_of(gv[i], z, a);
-        hp[i] = rp && rp[t0 + i] ? 0.f : h;
-        h = fmaf(a, hp[i], z * xv[i]);
-      }
-    }
+    for (int q = 0; q < kLook; q++)
 #pragma unroll
-    for (int i = kTS - 1; i >= 0; i--) {
-      if (t0 + i >= p.L) continue;
-      float ox = 0.f, og = 0.f;
-      if (t0 + i < n) {
-        float z, a;
-        gate_of(gv[i], z, a);
-        dh += yv[i];
-        ox = dh * z;
-        og = dh * (xv[i] - hp[i]) * z * a;
-        dh = rp && rp[t0 + i] ? 0.f : dh * a;
+      for (int v = 0; v < VEC; v++) w[q][v] = peek(word + (j - q > 0 ? j - q : 0) * stride + v);
+#pragma unroll
+    for (int q = 0; q < kLook; q++) {
+      all = true;
+#pragma unroll
+      for (int v = 0; v < VEC; v++) {
+        if (done[v]) continue;
+        while (uint32_t(w[q][v] >> 32) == 0xFFFFFFFFu) {
+          __builtin_amdgcn_s_sleep(1);
+          w[q][v] = peek(word + (j - q > 0 ? j - q : 0) * stride + v);
+        }
+        const float h = __uint_as_float(uint32_t(w[q][v]));
+        if (uint32_t(w[q][v] >> 32) == kFinished) {  // segment 0 always comes to be
+          out[v] = apply(acc[v], h);
+          done[v] = true;
+        } else {
+          acc[v] = then(Map{__uint_as_float(uint32_t(w[q][v] >> 32)), h}, acc[v]);
+          if (acc[v].A == 0.f) {
+            out[v] = acc[v].H;
+            done[v] = true;
+          }
+        }
+        all = all && done[v];
       }
-      dx[b * p.dsb + (t0 + i) * p.dst + d] = from_f32<T>(ox);
-      dg[b * p.dsb + (t0 + i) * p.dst + d] = from_f32<T>(og);
+      if (all) break;
     }
   }
-  if (p.dh0) p.dh0[b * p.D + d] = dh;
+}
+
+struct ScanPlace {
+  int64_t b, d, seg;
+  int wave, lane, waves;
+};
+
+// Which (sequence, channels, segment) this workgroup has. Consecutive tickets are different chains, so a chain's
+// segments start as far apart as the number of chains allows.
+template <int VEC>
+__device__ __forceinline__ ScanPlace scan_place(const ScanArgs& p, uint32_t* __restrict__ ticket, uint32_t* shared) {
+  uint32_t id = blockIdx.x;
+  if (ticket != nullptr) {
+    if (threadIdx.x == 0) *shared = atomicAdd(ticket, 1u);
+    __syncthreads();
+    id = __builtin_amdgcn_readfirstlane(*shared);
+  }
+  const uint32_t tiles = uint32_t((p.D + kWave * VEC - 1) / (kWave * VEC)), chains = uint32_t(p.B) * tiles;
+  const uint32_t seg = id / chains, c = id - seg * chains, b = c / tiles;
+  ScanPlace s;
+  s.seg = seg;
+  s.b = b;
+  s.lane = threadIdx.x % kWave;
+  s.wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  s.waves = blockDim.x / kWave;
+  s.d = (int64_t(c - b * tiles) * kWave + s.lane) * VEC;
+  return s;
+}
+
+// Bits of the steps t0 .. t0 + K - 1 (below n) that have a reset; the same in every lane.
+template <int K>
+__device__ __forceinline__ uint32_t reset_bits(const uint8_t* __restrict__ resets, int64_t at, int lane, int cnt) {
+  if (resets == nullptr) return 0;
+  return uint32_t(__ballot(lane < cnt && resets[at + lane] != 0));
+}
+
+template <typename T, int VEC, int K>
+__device__ __forceinline__ void load_rows(const T* __restrict__ p, int64_t stride, int cnt, VecOf<T, VEC> (&r)[K]) {
+  if (cnt == K) {
+#pragma unroll
+    for (int i = 0; i < K; i++) r[i] = *reinterpret_cast<const VecOf<T, VEC>*>(p + i * stride);
+  } else {
+#pragma unroll
+    for (int i = 0; i < K; i++)
+      if (i < cnt) r[i] = *reinterpret_cast<const VecOf<T, VEC>*>(p + i * stride);
+  }
+}
+
+// The state that enters each wave's chunk, from the waves' compositions and what enters the workgroup. `first` is the
+// wave whose chunk comes first in the order of the recurrence, `step` = +1 or -1 the direction; *last gets the state
+// behind the workgroup (in wave 0).
+template <int VEC>
+__device__ __forceinline__ void exchange(const ScanArgs& p, const ScanPlace& s, bool forward, int64_t seg, int64_t nseg,
+                                         const float* __restrict__ start, uint64_t* __restrict__ words,
+                                         const Map (&mine)[VEC], float (&in)[VEC], float (&last)[VEC]) {
+  __shared__ Map maps[kScanWaves][kWave * VEC];
+  __shared__ float entry[kWave * VEC];
+  const bool live = s.d < p.D;
+#pragma unroll
+  for (int v = 0; v < VEC; v++) maps[s.wave][s.lane * VEC + v] = mine[v];
+  __syncthreads();
+  const int order = forward ? s.wave : s.waves - 1 - s.wave;  // chunks before mine
+  if (s.wave == 0) {
+    const int64_t dp = (p.D + 127) / 128 * 128, stride = p.B * dp;
+    uint64_t* word = words + s.b * dp + s.d;
+    Map all[VEC];
+    float e[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+      all[v] = Map{1.f, 0.f};
+      for (int k = 0; k < s.waves; k++)
+        all[v] = then(all[v], maps[forward ? k : s.waves - 1 - k][s.lane * VEC + v]);
+      e[v] = 0.f;
+      if (live && seg > 0) publish(word + seg * stride + v, pack(all[v].A, all[v].H));
+      if (live && seg == 0 && start) e[v] = start[s.b * p.D + s.d + v];
+    }
+    if (live && seg > 0) look_back<VEC>(word, seg, stride, e);
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+      last[v] = apply(all[v], e[v]);
+      if (live && nseg > 1) publish(word + seg * stride + v, pack(__uint_as_float(kFinished), last[v]));
+      entry[s.lane * VEC + v] = e[v];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < VEC; v++) {
+    in[v] = entry[s.lane * VEC + v];
+    for (int k = 0; k < order; k++) in[v] = apply(maps[forward ? k : s.waves - 1 - k][s.lane * VEC + v], in[v]);
+  }
+}
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void k_scan_fwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
+                                                  T* __restrict__ y, int64_t nseg, uint64_t* __restrict__ words,
+                                                  uint32_t* __restrict__ ticket) {
+  constexpr int K = chunk_steps<T>();
+  __shared__ uint32_t shared;
+  const ScanPlace s = scan_place<VEC>(p, ticket, &shared);
+  const bool live = s.d < p.D;
+  const int64_t n = length_of(p.lengths, s.b, p.L), nck = (p.L + K - 1) / K, ck = s.seg * s.waves + s.wave, t0 = ck * K;
+  const int rows = int(max(int64_t(0), min(int64_t(K), p.L - t0))), cnt = int(max(int64_t(0), min(int64_t(K), n - t0)));
+  VecOf<T, VEC> xr[K], gr[K];
+  if (live) {
+    load_rows<T, VEC, K>(x + s.b * p.xsb + t0 * p.xst + s.d, p.xst, cnt, xr);
+    load_rows<T, VEC, K>(g + s.b * p.gsb + t0 * p.gst + s.d, p.gst, cnt, gr);
+  }
+  const uint32_t rb = reset_bits<K>(p.resets, s.b * p.L + t0, s.lane, cnt);
+  float ca[K][VEC], ch[K][VEC];  // the composition up to each step
+  Map m[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < K; i++) {
+    const bool drop = (rb >> i) & 1, dropped = (rb & ((2u << i) - 1)) != 0;
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+      if (i < cnt) {
+        float z, a;
+        gate_of(to_f32(gr[i].v[v]), z, a);
+        const float u = z * to_f32(xr[i].v[v]);
+        m[v].H = drop ? u : fmaf(a, m[v].H, u);
+        m[v].A = dropped ? 0.f : fmaxf(m[v].A * a, kTiny);
+      }
+      ca[i][v] = m[v].A;
+      ch[i][v] = m[v].H;
+    }
+  }
+  float in[VEC], last[VEC];
+  exchange<VEC>(p, s, true, s.seg, nseg, p.h0, words, m, in, last);
+  if (!live) return;
+  if (s.wave == 0 && s.seg == nseg - 1) store_vec<float, VEC>(p.h_last + s.b * p.D + s.d, last);
+  if (rows > 0 && p.ckpt) store_vec<float, VEC>(p.ckpt + (s.b * nck + ck) * p.D + s.d, in);
+  T* yp = y + (s.b * p.L + t0) * p.D + s.d;
+#pragma unroll
+  for (int i = 0; i < K; i++) {
+    if (i < rows) {
+      float o[VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; v++) o[v] = i < cnt ? apply(Map{ca[i][v], ch[i][v]}, in[v]) : 0.f;
+      store_vec<T, VEC>(yp + i * p.D, o);
+    }
+  }
+}
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void k_scan_bwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
+                                                  const T* __restrict__ dy, T* __restrict__ dx, T* __restrict__ dg,
+                                                  int64_t nseg, uint64_t* __restrict__ words,
+                                                  uint32_t* __restrict__ ticket) {
+  constexpr int K = chunk_steps<T>();
+  __shared__ uint32_t shared;
+  const ScanPlace s = scan_place<VEC>(p, ticket, &shared);
+  const bool live = s.d < p.D;
+  const int64_t seg = nseg - 1 - s.seg;  // time runs backwards along the tickets
+  const int64_t n = length_of(p.lengths, s.b, p.L), nck = (p.L + K - 1) / K, ck = seg * s.waves + s.wave, t0 = ck * K;
+  const int rows = int(max(int64_t(0), min(int64_t(K), p.L - t0))), cnt = int(max(int64_t(0), min(int64_t(K), n - t0)));
+  VecOf<T, VEC> xr[K], gr[K], yr[K];
+  float h[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; v++) h[v] = 0.f;
+  if (live) {
+    load_rows<T, VEC, K>(x + s.b * p.xsb + t0 * p.xst + s.d, p.xst, cnt, xr);
+    load_rows<T, VEC, K>(g + s.b * p.gsb + t0 * p.gst + s.d, p.gst, cnt, gr);
+    if (dy) load_rows<T, VEC, K>(dy + s.b * p.ysb + t0 * p.yst + s.d, p.yst, cnt, yr);
+    if (rows > 0) load_vec<float, VEC>(p.ckpt + (s.b * nck + ck) * p.D + s.d, h);
+  }
+  const uint32_t rb = reset_bits<K>(p.resets, s.b * p.L + t0, s.lane, cnt);
+  float zz[K][VEC], aa[K][VEC], cc[K][VEC];  // z, 1 - z and dg / dh of each step
+#pragma unroll
+  for (int i = 0; i < K; i++) {
+    const bool drop = (rb >> i) & 1;
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+      if (i < cnt) {
+        gate_of(to_f32(gr[i].v[v]), zz[i][v], aa[i][v]);
+        const float xv = to_f32(xr[i].v[v]), prev = drop ? 0.f : h[v];
+        cc[i][v] = (xv - prev) * (zz[i][v] * aa[i][v]);
+        h[v] = fmaf(aa[i][v], prev, zz[i][v] * xv);
+      }
+    }
+  }
+  // what reaches the state behind step i from outside the chunk: aa[i] times, and from inside: dh[i]
+  float dh[K][VEC];
+  Map m[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
+#pragma unroll
+  for (int i = K - 1; i >= 0; i--) {
+    const bool drop = (rb >> i) & 1, dropped = (rb >> i) != 0;
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+      if (i < cnt) {
+        const float d = m[v].H + (dy ? to_f32(yr[i].v[v]) : 0.f), a = aa[i][v];
+        dh[i][v] = d;
+        aa[i][v] = m[v].A;
+        m[v].H = drop ? 0.f : a * d;
+        m[v].A = dropped ? 0.f : fmaxf(m[v].A * a, kTiny);
+      }
+    }
+  }
+  float in[VEC], last[VEC];
+  exchange<VEC>(p, s, false, s.seg, nseg, p.dh_last, words, m, in, last);
+  if (!live) return;
+  if (p.dh0 && s.wave == 0 && s.seg == nseg - 1) store_vec<float, VEC>(p.dh0 + s.b * p.D + s.d, last);
+  T *xp = dx + s.b * p.dsb + t0 * p.dst + s.d, *gp = dg + s.b * p.dsb + t0 * p.dst + s.d;
+#pragma unroll
+  for (int i = 0; i < K; i++) {
+    if (i < rows) {
+      float ox[VEC], og[VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; v++) {
+        const float d = i < cnt ? apply(Map{aa[i][v], dh[i][v]}, in[v]) : 0.f;
+        ox[v] = i < cnt ? d * zz[i][v] : 0.f;
+        og[v] = i < cnt ? d * cc[i][v] : 0.f;
+      }
+      store_vec<T, VEC>(xp + i * p.dst, ox);
+      store_vec<T, VEC>(gp + i * p.dst, og);
+    }
+  }
 }
 
 template <typename T>
@@ -138,23 +371,74 @@ __global__ __launch_bounds__(256) void k_scan_step(const T* __restrict__ x, int6
   y[i] = from_f32<T>(hn);
 }
 
-dim3 scan_grid(const ScanArgs& p, const char* who) {
-  const int64_t gx = (p.D + kWave - 1) / kWave;
-  if (gx > (int64_t(1) << 31) - 1 || p.B > 65535) throw std::invalid_argument(std::string(who) + ": too many rows");
-  return dim3(uint32_t(gx), uint32_t(p.B));
+struct ScanPlan {
+  int waves = 1;
+  int64_t nseg = 1, blocks = 0;
+};
+
+int chunk_of(int type) { return type == kF32 ? chunk_steps<float>() : chunk_steps<f16_t>(); }
+
+ScanPlan scan_plan(const ScanArgs& p, int type, int vec, const char* who) {
+  ScanPlan s;
+  const int64_t chunks = std::max<int64_t>(1, (p.L + chunk_of(type) - 1) / chunk_of(type));
+  s.waves = int(std::min<int64_t>(kScanWaves, chunks));
+  s.nseg = (chunks + s.waves - 1) / s.waves;
+  const int64_t tiles = (p.D + kWave * vec - 1) / (kWave * vec);
+  if (p.B > (int64_t(1) << 31) / tiles / s.nseg) throw std::invalid_argument(std::string(who) + ": too many elements");
+  s.blocks = p.B * tiles * s.nseg;
+  return s;
+}
+
+int64_t scan_words(const ScanArgs& p, const ScanPlan& s) { return s.nseg == 1 ? 0 : s.nseg * p.B * ((p.D + 127) / 128 * 128); }
+
+// Two channels a lane where every row of every tensor starts at a multiple of two elements.
+template <typename T>
+bool pairs(const ScanArgs& p, std::initializer_list<const void*> ptrs) {
+  if ((p.D | p.xsb | p.xst | p.gsb | p.gst | p.ysb | p.yst | p.dsb | p.dst) % 2) return false;
+  for (const void* q : ptrs)
+    if (!vec_aligned<T, 2>(q)) return false;
+  return true;
+}
+
+// Words not yet written, ticket 0: before a pass whose workgroups hand the state on.
+uint32_t* scan_begin(const ScanArgs& p, const ScanPlan& s, const char* who, hipStream_t stream) {
+  if (s.nseg == 1) return nullptr;
+  if (p.workspace == nullptr) throw std::invalid_argument(std::string(who) + ": no workspace");
+  const int64_t n = scan_words(p, s);
+  uint64_t* words = static_cast<uint64_t*>(p.workspace);
+  uint32_t* ticket = reinterpret_cast<uint32_t*>(words + n);
+  hipLaunchKernelGGL(k_scan_init, dim3(uint32_t(std::min<int64_t>((n + 1023) / 1024, 2048))), dim3(256), 0, stream, words,
+                     n, ticket);
+  RMM_HIP_CHECK(hipGetLastError());
+  return ticket;
 }
 
 }  // namespace
 
-int64_t gated_scan_checkpoints(int64_t L) { return (L + kTS - 1) / kTS; }
+int64_t gated_scan_checkpoints(int64_t L, int type) { return (L + chunk_of(type) - 1) / chunk_of(type); }
+
+int64_t gated_scan_workspace(int64_t B, int64_t L, int64_t D, int type) {
+  ScanArgs p;
+  p.B = B, p.L = L, p.D = D;
+  if (B <= 0 || D <= 0) return 0;
+  return scan_words(p, scan_plan(p, type, 1, "gated_scan")) * int64_t(sizeof(uint64_t)) + 64;
+}
 
 void gated_scan_fwd(const ScanArgs& p, const void* x, const void* g, void* y, int type, hipStream_t stream) {
   if (p.B <= 0 || p.D <= 0) return;
-  const dim3 grid = scan_grid(p, "gated_scan");
   dispatch_type(type, "gated_scan", [&](auto tag) {
     using T = decltype(tag);
-    hipLaunchKernelGGL((k_scan_fwd<T>), grid, dim3(kWave), 0, stream, p, static_cast<const T*>(x),
-                       static_cast<const T*>(g), static_cast<T*>(y));
+    const bool two = pairs<T>(p, {x, g, y});
+    const ScanPlan s = scan_plan(p, type, two ? 2 : 1, "gated_scan");
+    uint32_t* ticket = scan_begin(p, s, "gated_scan", stream);
+    const dim3 grid(uint32_t(s.blocks)), block(uint32_t(s.waves * kWave));
+    const T *xp = static_cast<const T*>(x), *gp = static_cast<const T*>(g);
+    T* yp = static_cast<T*>(y);
+    uint64_t* words = static_cast<uint64_t*>(p.workspace);
+    if (two)
+      hipLaunchKernelGGL((k_scan_fwd<T, 2>), grid, block, 0, stream, p, xp, gp, yp, s.nseg, words, ticket);
+    else
+      hipLaunchKernelGGL((k_scan_fwd<T, 1>), grid, block, 0, stream, p, xp, gp, yp, s.nseg, words, ticket);
   });
   RMM_HIP_CHECK(hipGetLastError());
 }
@@ -163,11 +447,19 @@ void gated_scan_bwd(const ScanArgs& p, const void* x, const void* g, const void*
                     hipStream_t stream) {
   if (p.B <= 0 || p.D <= 0) return;
   if (p.L > 0 && p.ckpt == nullptr) throw std::invalid_argument("gated_scan backward: no saved states");
-  const dim3 grid = scan_grid(p, "gated_scan backward");
   dispatch_type(type, "gated_scan backward", [&](auto tag) {
     using T = decltype(tag);
-    hipLaunchKernelGGL((k_scan_bwd<T>), grid, dim3(kWave), 0, stream, p, static_cast<const T*>(x),
-                       static_cast<const T*>(g), static_cast<const T*>(dy), static_cast<T*>(dx), static_cast<T*>(dg));
+    const bool two = pairs<T>(p, {x, g, dy, dx, dg});
+    const ScanPlan s = scan_plan(p, type, two ? 2 : 1, "gated_scan backward");
+    uint32_t* ticket = scan_begin(p, s, "gated_scan backward", stream);
+    const dim3 grid(uint32_t(s.blocks)), block(uint32_t(s.waves * kWave));
+    const T *xp = static_cast<const T*>(x), *gp = static_cast<const T*>(g), *yp = static_cast<const T*>(dy);
+    T *dxp = static_cast<T*>(dx), *dgp = static_cast<T*>(dg);
+    uint64_t* words = static_cast<uint64_t*>(p.workspace);
+    if (two)
+      hipLaunchKernelGGL((k_scan_bwd<T, 2>), grid, block, 0, stream, p, xp, gp, yp, dxp, dgp, s.nseg, words, ticket);
+    else
+      hipLaunchKernelGGL((k_scan_bwd<T, 1>), grid, block, 0, stream, p, xp, gp, yp, dxp, dgp, s.nseg, words, ticket);
   });
   RMM_HIP_CHECK(hipGetLastError());
 }

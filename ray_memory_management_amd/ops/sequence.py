@@ -309,6 +309,10 @@ def _scan_cpu(x, gate, h0, resets, lengths):
     return (torch.stack(ys, dim=1) if L else x.new_zeros((B, 0, D), dtype=st)), h
 
 
+def _scan_workspace(h, B, L, D, x):
+    return torch.empty(h.gated_scan_workspace(B, L, D, _CODE[x.dtype]), dtype=torch.uint8, device=x.device)
+
+
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, h0, resets, lengths):
@@ -326,11 +330,12 @@ class _GatedScan(torch.autograd.Function):
         h_last = torch.empty((B, D), dtype=torch.float32, device=x.device)
         ckpt = None
         if any(ctx.needs_input_grad):
-            ckpt = torch.empty((B, h.gated_scan_checkpoints(L), D), dtype=torch.float32, device=x.device)
+            ckpt = torch.empty((B, h.gated_scan_checkpoints(L, _CODE[x.dtype]), D), dtype=torch.float32, device=x.device)
+        ws = _scan_workspace(h, B, L, D, x)
         with _device(x):
             h.gated_scan_fwd(x.data_ptr(), gp, y.data_ptr(), _CODE[x.dtype], (B, L, D),
                              (x.stride(0), x.stride(1), *gs), _ptr(h0), _ptr(resets), _ptr(lengths), _ptr(ckpt),
-                             h_last.data_ptr(), _stream(x))
+                             h_last.data_ptr(), ws.data_ptr(), _stream(x))
         ctx.save_for_backward(x, g, resets, lengths, ckpt)
         return y, h_last
 
@@ -353,10 +358,11 @@ class _GatedScan(torch.autograd.Function):
         dy = None if dy is None else _rows(dy)
         dh = None if dh is None else dh.contiguous()
         ys = (0, 0) if dy is None else (dy.stride(0), dy.stride(1))
+        ws = _scan_workspace(h, B, L, D, x)
         with _device(x):
             h.gated_scan_bwd(x.data_ptr(), gp, _ptr(dy), dx.data_ptr(), dgp, _CODE[x.dtype], (B, L, D),
                              (x.stride(0), x.stride(1), *gs, *ys, *ds), _ptr(resets), _ptr(lengths), _ptr(ckpt),
-                             _ptr(dh), _ptr(dh0), _stream(x))
+                             _ptr(dh), _ptr(dh0), ws.data_ptr(), _stream(x))
         return dx, dg, dh0, None, None
 
 

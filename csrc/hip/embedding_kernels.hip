@@ -54,8 +54,109 @@ __global__ __launch_bounds__(256) void k_embed_fwd(const TI* __restrict__ ids, c
 }
 
 // ------------------------------------------------------------------------------------------ sort
+// Stable least-significant-digit radix sort of (key, position). Batches of up to kSmall ids are sorted by one workgroup
+// in LDS (one launch); larger ones in tiles, a count and a scatter launch for each digit of up to 9 bits.
+
+// Lanes of this wave whose digit equals mine (inactive lanes excluded).
+__device__ __forceinline__ uint64_t match_digit(uint32_t d, int bits, bool active) {
+  uint64_t m = __ballot(active);
+  for (int b = 0; b < bits; b++) {
+    const bool one = (d >> b) & 1;
+    const uint64_t v = __ballot(one && active);
+    m &= one ? v : ~v;
+  }
+  return m;
+}
+
+// Orders LDS accesses of one wave (its lanes run in step; this holds the compiler to that order).
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+// The slot of this lane's element: its digit's running slot (moved on for the whole wave) plus its rank among the lanes
+// with the same digit, in lane order.
+__device__ __forceinline__ uint32_t take_slot(uint32_t* slots, uint32_t d, int bits, int lane, bool active) {
+  const uint64_t same = match_digit(d, bits, active);
+  uint32_t at = 0;
+  if (active) {
+    const int rank = __popcll(same & ((uint64_t(1) << lane) - 1));
+    at = slots[d] + rank;
+    wave_fence();  // all lanes have read the slot before its first lane moves it on
+    if (rank == 0) slots[d] += __popcll(same);
+  }
+  wave_fence();
+  return at;
+}
+
+constexpr int kSmall = 8192, kSmallThreads = 1024, kSmallWaves = kSmallThreads / kWave, kSmallBits = 8;
+constexpr int kSmallRadix = 1 << kSmallBits;
+
+template <typename TI>
+__global__ __launch_bounds__(kSmallThreads) void k_sort_small(const TI* __restrict__ ids, int n, int64_t V, int64_t pad,
+                                                              int passes, int bits, uint32_t* __restrict__ okeys,
+                                                              uint32_t* __restrict__ opos) {
+  __shared__ uint32_t key[2][kSmall];
+  __shared__ uint16_t pos[2][kSmall];
+  __shared__ uint32_t slot[kSmallWaves][kSmallRadix];
+  __shared__ uint32_t wsum[kSmallWaves];
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, radix = 1 << bits;
+  const int seg = (n + kSmallThreads - 1) / kSmallThreads * kWave, lo = min(n, wave * seg), hi = min(n, lo + seg);
+  for (int i = tid; i < n; i += kSmallThreads) {
+    key[0][i] = embed_key(ids[i], V, pad);
+    pos[0][i] = uint16_t(i);
+  }
+  for (int s = 0; s < passes; s++) {
+    const int from = s & 1, to = from ^ 1, shift = s * bits;
+    for (int r = lane; r < radix; r += kWave) slot[wave][r] = 0;
+    __syncthreads();
+    for (int i = lo + lane; i < hi; i += kWave) atomicAdd(&slot[wave][(key[from][i] >> shift) & (radix - 1)], 1u);
+    __syncthreads();
+    // exclusive sums in the order (digit, wave): 4 threads a digit, 4 waves each
+    const int d = tid / 4, w0 = tid % 4 * 4;
+    uint32_t c[4] = {}, sum = 0;
+    if (d < radix) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        c[k] = slot[w0 + k][d];
+        sum += c[k];
+      }
+    }
+    uint32_t incl = sum;
+    for (int off = 1; off < kWave; off <<= 1) {
+      const uint32_t up = __shfl_up(incl, off);
+      if (lane >= off) incl += up;
+    }
+    if (lane == kWave - 1) wsum[wave] = incl;
+    __syncthreads();
+    uint32_t at = incl - sum;
+    for (int w = 0; w < wave; w++) at += wsum[w];
+    if (d < radix) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        slot[w0 + k][d] = at;
+        at += c[k];
+      }
+    }
+    __syncthreads();
+    for (int i0 = lo; i0 < hi; i0 += kWave) {
+      const int i = i0 + lane;
+      const bool active = i < hi;
+      const uint32_t k = active ? key[from][i] : 0u;
+      const uint32_t to_slot = take_slot(slot[wave], (k >> shift) & (radix - 1), bits, lane, active);
+      if (active) {
+        if (s == passes - 1) {
+          okeys[to_slot] = k;
+          opos[to_slot] = pos[from][i];
+        } else {
+          key[to][to_slot] = k;
+          pos[to][to_slot] = pos[from][i];
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
 constexpr int kSortThreads = 256, kSortWaves = kSortThreads / kWave, kMaxBits = 9, kMaxRadix = 1 << kMaxBits;
-constexpr int kMaxTiles = 256;
+constexpr int kMaxTiles = 256, kMinTile = 1024;
 
 // Digit counts of each tile: counts[tile][radix].
 template <typename TI>
@@ -75,20 +176,6 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_hist(const TI* __restrict
   for (int r = threadIdx.x; r < radix; r += kSortThreads) counts[int64_t(blockIdx.x) * radix + r] = hist[r];
 }
 
-// Lanes of this wave whose digit equals mine (inactive lanes excluded).
-__device__ __forceinline__ uint64_t match_digit(uint32_t d, int bits, bool active) {
-  uint64_t m = __ballot(active);
-  for (int b = 0; b < bits; b++) {
-    const bool one = (d >> b) & 1;
-    const uint64_t v = __ballot(one && active);
-    m &= one ? v : ~v;
-  }
-  return m;
-}
-
-// Orders LDS accesses of one wave (its lanes run in step; this holds the compiler to that order).
-__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
-
 // One stable pass: tile after tile, wave after wave, round after round, lane after lane is the input order,
 // and the slot of an element is (smaller digits anywhere) + (same digit in earlier tiles, waves, rounds, lanes).
 template <typename TI>
@@ -98,28 +185,39 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(const TI* __restr
                                                                int64_t V, int64_t pad, int shift, int bits,
                                                                const uint32_t* __restrict__ counts,
                                                                uint32_t* __restrict__ okeys, uint32_t* __restrict__ opos) {
-  __shared__ uint32_t base[kMaxRadix];                // slot of the digit's first element of this tile
-  __shared__ uint32_t whist[kSortWaves][kMaxRadix];   // counts, then running slots, of each wave
+  __shared__ uint32_t base[kMaxRadix];               // slot of the digit's first element of this tile
+  __shared__ uint32_t slot[kSortWaves][kMaxRadix];   // counts, then running slots, of each wave
   __shared__ uint32_t wsum[kSortWaves];
   const int radix = 1 << bits, tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
   const int64_t lo = int64_t(blockIdx.x) * tile, hi = min(n, lo + tile);
-  const int64_t seg = tile / kSortWaves, wlo = lo + wave * seg, whi = min(hi, wlo + seg);
-  for (int r = lane; r < radix; r += kWave) whist[wave][r] = 0;
+  const int64_t seg = tile / kSortWaves, wlo = min(hi, lo + wave * seg), whi = min(hi, wlo + seg);
+  for (int r = lane; r < radix; r += kWave) slot[wave][r] = 0;
+  wave_fence();
   for (int64_t i = wlo + lane; i < whi; i += kWave) {  // this wave's counts
     const uint32_t k = ids ? embed_key(ids[i], V, pad) : keys[i];
-    atomicAdd(&whist[wave][(k >> shift) & (radix - 1)], 1u);
+    atomicAdd(&slot[wave][(k >> shift) & (radix - 1)], 1u);
   }
   // digits 2t and 2t+1 belong to thread t: totals over all tiles, and the part of the earlier tiles
   const int r0 = 2 * tid;
   uint32_t total[2] = {0, 0}, before[2] = {0, 0};
+  if (r0 < radix) {
+    const uint2* col = reinterpret_cast<const uint2*>(counts + r0);  // radix is even: bits >= 1
+    const int tiles = int(gridDim.x), mine = int(blockIdx.x);
+    int b = 0;
+    for (; b + 8 <= tiles; b += 8) {
+      uint2 c[8];
 #pragma unroll
-  for (int k = 0; k < 2; k++) {
-    if (r0 + k < radix) {
-      for (uint32_t b = 0; b < gridDim.x; b++) {
-        const uint32_t c = counts[int64_t(b) * radix + r0 + k];
-        total[k] += c;
-        if (b < blockIdx.x) before[k] += c;
+      for (int k = 0; k < 8; k++) c[k] = col[int64_t(b + k) * (radix / 2)];
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        total[0] += c[k].x, total[1] += c[k].y;
+        if (b + k < mine) before[0] += c[k].x, before[1] += c[k].y;
       }
+    }
+    for (; b < tiles; b++) {
+      const uint2 c = col[int64_t(b) * (radix / 2)];
+      total[0] += c.x, total[1] += c.y;
+      if (b < mine) before[0] += c.x, before[1] += c.y;
     }
   }
   uint32_t incl = total[0] + total[1];
@@ -131,14 +229,16 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(const TI* __restr
   __syncthreads();
   uint32_t excl = incl - total[0] - total[1];
   for (int w = 0; w < wave; w++) excl += wsum[w];
-  if (r0 < radix) base[r0] = excl + before[0];
-  if (r0 + 1 < radix) base[r0 + 1] = excl + total[0] + before[1];
+  if (r0 < radix) {
+    base[r0] = excl + before[0];
+    base[r0 + 1] = excl + total[0] + before[1];
+  }
   __syncthreads();
   for (int r = tid; r < radix; r += kSortThreads) {
     uint32_t at = base[r];
     for (int w = 0; w < kSortWaves; w++) {
-      const uint32_t c = whist[w][r];
-      whist[w][r] = at;
+      const uint32_t c = slot[w][r];
+      slot[w][r] = at;
       at += c;
     }
   }
@@ -147,21 +247,29 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(const TI* __restr
     const int64_t i = i0 + lane;
     const bool active = i < whi;
     const uint32_t k = !active ? 0u : ids ? embed_key(ids[i], V, pad) : keys[i];
-    const uint32_t d = (k >> shift) & (radix - 1);
-    const uint64_t same = match_digit(d, bits, active);
+    const uint32_t at = take_slot(slot[wave], (k >> shift) & (radix - 1), bits, lane, active);
     if (active) {
-      const int rank = __popcll(same & ((uint64_t(1) << lane) - 1));
-      const uint32_t at = whist[wave][d] + rank;
-      wave_fence();  // all lanes have read the slot before its first lane moves it on
-      if (rank == 0) whist[wave][d] += __popcll(same);
       okeys[at] = k;
       opos[at] = ids ? uint32_t(i) : pos[i];
     }
-    wave_fence();
   }
 }
 
 // ------------------------------------------------------------------------------------------ segment sums
+// The sorted positions are cut into pieces of one length, and 2^lpr lanes walk a piece for a chunk of 2^lpr VEC columns:
+// the reads of dy are spread evenly however the tokens are distributed. A token whose segment lies inside a piece is
+// written at once. One that crosses pieces leaves its sum in each: part[2p] for the segment that entered piece p,
+// part[2p + 1] for one that starts in p and goes on; k_embed_join adds those up in order. Rows without a token are
+// written by the same launch's further workgroups.
+struct SumPlan {
+  int64_t piece = 0, pieces = 0;  // positions in a piece, pieces
+  int lpr = 0;
+  int64_t chunks = 0;             // of columns
+};
+
+constexpr int kAhead = 8;        // rows of dy in flight per lane
+constexpr int kZeroRows = 64;    // rows that a zero-writing workgroup looks at
+
 __device__ __forceinline__ uint32_t lower_bound(const uint32_t* __restrict__ keys, uint32_t n, uint32_t v) {
   uint32_t lo = 0, hi = n;
   while (lo < hi) {
@@ -171,25 +279,122 @@ __device__ __forceinline__ uint32_t lower_bound(const uint32_t* __restrict__ key
   return lo;
 }
 
-template <typename TW, typename TO, int VEC>
-__global__ __launch_bounds__(256) void k_embed_rows(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
-                                                    uint32_t n, const TO* __restrict__ dy, int64_t dys,
-                                                    TW* __restrict__ dw, int64_t V, int64_t D, float scale, int lpr) {
-  const int lane = threadIdx.x & ((1 << lpr) - 1);
-  const int64_t v = (int64_t(blockIdx.x) * 256 + threadIdx.x) >> lpr;
-  if (v >= V) return;
-  const uint32_t first = lower_bound(keys, n, uint32_t(v));
-  for (int64_t c = int64_t(lane) * VEC; c < D; c += int64_t(VEC) << lpr) {
-    float acc[VEC] = {};
-    for (uint32_t j = first; j < n && keys[j] == uint32_t(v); j++) {
-      float x[VEC];
-      load_vec<TO, VEC>(dy + int64_t(pos[j]) * dys + c, x);
+template <typename TW, int VEC>
+__device__ __forceinline__ void write_row(TW* __restrict__ dw, int64_t at, const float (&acc)[VEC], float scale) {
+  float o[VEC];
 #pragma unroll
-      for (int k = 0; k < VEC; k++) acc[k] += x[k];
+  for (int k = 0; k < VEC; k++) o[k] = acc[k] * scale;
+  store_vec<TW, VEC>(dw + at, o);
+}
+
+template <typename TW, typename TO, int VEC>
+__global__ __launch_bounds__(256) void k_embed_sum(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
+                                                   uint32_t n, const TO* __restrict__ dy, int64_t dys,
+                                                   TW* __restrict__ dw, float* __restrict__ part, int64_t V, int64_t D,
+                                                   float scale, SumPlan s, uint32_t sum_blocks) {
+  if (blockIdx.x >= sum_blocks) {
+    __shared__ bool used[kZeroRows];
+    const int64_t v0 = int64_t(blockIdx.x - sum_blocks) * kZeroRows;
+    const int rows = int(min(int64_t(kZeroRows), V - v0));
+    if (threadIdx.x < rows) {
+      const uint32_t v = uint32_t(v0 + threadIdx.x), at = lower_bound(keys, n, v);
+      used[threadIdx.x] = at < n && keys[at] == v;
+    }
+    __syncthreads();
+    float zero[VEC] = {};
+    const int lane = threadIdx.x & ((1 << s.lpr) - 1);
+    for (int r = threadIdx.x >> s.lpr; r < rows; r += 256 >> s.lpr) {
+      if (used[r]) continue;
+      for (int64_t c = int64_t(lane) * VEC; c < D; c += int64_t(VEC) << s.lpr) store_vec<TW, VEC>(dw + (v0 + r) * D + c, zero);
+    }
+    return;
+  }
+  const int64_t unit = (int64_t(blockIdx.x) * 256 + threadIdx.x) >> s.lpr;
+  const int64_t p = unit / s.chunks;
+  const int64_t c = ((unit - p * s.chunks) << s.lpr) * VEC + (threadIdx.x & ((1 << s.lpr) - 1)) * VEC;
+  if (p >= s.pieces || c >= D) return;
+  const uint32_t lo = uint32_t(p * s.piece), hi = uint32_t(min(int64_t(n), int64_t(lo) + s.piece));
+  uint32_t cur = keys[lo];
+  bool entered = lo > 0 && keys[lo - 1] == cur;  // the segment at hand began in an earlier piece
+  const bool leaves = hi < n && keys[hi] == keys[hi - 1];
+  float acc[VEC] = {};
+  for (uint32_t j0 = lo; j0 < hi; j0 += kAhead) {
+    uint32_t k[kAhead];
+    VecOf<TO, VEC> row[kAhead];
+#pragma unroll
+    for (int q = 0; q < kAhead; q++) {
+      const uint32_t j = min(j0 + q, hi - 1);
+      k[q] = keys[j];
+      row[q] = *reinterpret_cast<const VecOf<TO, VEC>*>(dy + int64_t(pos[j]) * dys + c);
     }
 #pragma unroll
-    for (int k = 0; k < VEC; k++) acc[k] *= scale;
-    store_vec<TW, VEC>(dw + v * D + c, acc);
+    for (int q = 0; q < kAhead; q++) {
+      if (j0 + q >= hi) break;
+      if (k[q] != cur) {
+        if (entered) {
+          store_vec<float, VEC>(part + 2 * p * D + c, acc);
+        } else {
+          write_row<TW, VEC>(dw, int64_t(cur) * D + c, acc, scale);
+        }
+        entered = false;
+        cur = k[q];
+#pragma unroll
+        for (int e = 0; e < VEC; e++) acc[e] = 0.f;
+      }
+      if (cur >= uint32_t(V)) return;  // only places without a gradient are left
+#pragma unroll
+      for (int e = 0; e < VEC; e++) acc[e] += to_f32(row[q].v[e]);
+    }
+  }
+  if (entered || leaves)
+    store_vec<float, VEC>(part + (2 * p + (entered ? 0 : 1)) * D + c, acc);
+  else
+    write_row<TW, VEC>(dw, int64_t(cur) * D + c, acc, scale);
+}
+
+// A workgroup per piece and chunk: the row whose segment starts in piece p and goes on behind it. The four waves add
+// up consecutive quarters of the pieces it covers; the quarters are joined in order.
+template <typename TW, int VEC>
+__global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__ keys, uint32_t n,
+                                                    const float* __restrict__ part, TW* __restrict__ dw, int64_t V,
+                                                    int64_t D, float scale, SumPlan s) {
+  __shared__ float quarter[4][kWave * VEC];
+  const int64_t p = blockIdx.x / s.chunks, ch = blockIdx.x - p * s.chunks;
+  const uint32_t lo = uint32_t(p * s.piece), hi = uint32_t(min(int64_t(n), int64_t(lo) + s.piece));
+  if (hi >= n) return;
+  const uint32_t v = keys[hi];
+  if (v >= uint32_t(V) || keys[hi - 1] != v || (lo > 0 && keys[lo - 1] == v)) return;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  int64_t count = 1;  // pieces covered: p and those whose first position still has token v
+  for (bool more = true; more; ) {
+    const int64_t at = (p + count + lane) * s.piece;
+    const int got = __popcll(__ballot(at < n && keys[at < n ? at : 0] == v));
+    count += got;
+    more = got == kWave;
+  }
+  const int64_t c = ((ch << s.lpr) + lane) * VEC;
+  const bool live = lane < (1 << s.lpr) && c < D;
+  const int64_t per = (count + 3) / 4, q0 = min(count, wave * per), q1 = min(count, q0 + per);
+  float acc[VEC] = {};
+  if (live) {
+    // piece p left its sum in slot 2p + 1, the pieces p + 1, p + 2, .. in slots 2p + 2, 2p + 4, ..
+#pragma unroll 8
+    for (int64_t q = q0; q < q1; q++) {
+      float x[VEC];
+      load_vec<float, VEC>(part + (2 * (p + q) + (q == 0 ? 1 : 0)) * D + c, x);
+#pragma unroll
+      for (int e = 0; e < VEC; e++) acc[e] += x[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; e++) quarter[wave][lane * VEC + e] = acc[e];
+  __syncthreads();
+  if (wave == 0 && live) {
+#pragma unroll
+    for (int w = 1; w < 4; w++)
+#pragma unroll
+      for (int e = 0; e < VEC; e++) acc[e] += quarter[w][lane * VEC + e];
+    write_row<TW, VEC>(dw, int64_t(v) * D + c, acc, scale);
   }
 }
 
@@ -206,6 +411,7 @@ uint32_t row_blocks(int64_t rows, int lpr, const char* who) {
 }
 
 struct SortPlan {
+  bool small = false;
   int64_t tile = 0;
   int tiles = 0, passes = 0, bits = 0;
 };
@@ -214,12 +420,27 @@ SortPlan sort_plan(int64_t n, int64_t V) {
   SortPlan p;
   int nb = 1;
   while ((int64_t(1) << nb) <= V) nb++;  // keys are 0 .. V
-  p.passes = (nb + kMaxBits - 1) / kMaxBits;
+  p.small = n <= kSmall;
+  const int most = p.small ? kSmallBits : kMaxBits;
+  p.passes = (nb + most - 1) / most;
   p.bits = (nb + p.passes - 1) / p.passes;
   const int64_t per = (n + kMaxTiles - 1) / kMaxTiles;
-  p.tile = std::max<int64_t>(2048, (per + kSortThreads - 1) / kSortThreads * kSortThreads);
+  p.tile = std::max<int64_t>(kMinTile, (per + kSortThreads - 1) / kSortThreads * kSortThreads);
   p.tiles = int((n + p.tile - 1) / p.tile);
   return p;
+}
+
+// Pieces of 16 to 128 positions: short enough that about 3000 waves walk them, long enough that the sums left between
+// pieces (8 bytes a column and piece, written and read) stay below the rows themselves.
+SumPlan sum_plan(int64_t n, int64_t D, int vec) {
+  SumPlan s;
+  s.lpr = std::min(6, lanes_log2(D, vec));
+  s.chunks = (D + (int64_t(vec) << s.lpr) - 1) / (int64_t(vec) << s.lpr);
+  const int64_t lanes = s.chunks << s.lpr;
+  s.piece = 16;
+  while (s.piece < 128 && n / (2 * s.piece) * lanes >= 3072 * kWave) s.piece *= 2;
+  s.pieces = (n + s.piece - 1) / s.piece;
+  return s;
 }
 
 template <typename TI, typename TW, typename TO>
@@ -245,9 +466,16 @@ void embed_sort(const TI* ids, int64_t n, int64_t V, int64_t pad, uint32_t* ws, 
                 const uint32_t** pos, hipStream_t stream) {
   const SortPlan p = sort_plan(n, V);
   uint32_t* buf[2][2] = {{ws, ws + n}, {ws + 2 * n, ws + 3 * n}};
-  uint32_t* counts = ws + 4 * n;
   const uint32_t *kin = nullptr, *pin = nullptr;
-  for (int s = 0; s < p.passes; s++) {
+  if (p.small) {
+    hipLaunchKernelGGL((k_sort_small<TI>), dim3(1), dim3(kSmallThreads), 0, stream, ids, int(n), V, pad, p.passes, p.bits,
+                       buf[0][0], buf[0][1]);
+    RMM_HIP_CHECK(hipGetLastError());
+    kin = buf[0][0];
+    pin = buf[0][1];
+  }
+  uint32_t* counts = ws + (4 * n + 1) / 2 * 2;  // read in pairs
+  for (int s = 0; s < p.passes && !p.small; s++) {
     const TI* src = s == 0 ? ids : nullptr;
     hipLaunchKernelGGL((k_sort_hist<TI>), dim3(p.tiles), dim3(kSortThreads), 0, stream, src, kin, n, p.tile, V, pad,
                        s * p.bits, p.bits, counts);
@@ -261,22 +489,38 @@ void embed_sort(const TI* ids, int64_t n, int64_t V, int64_t pad, uint32_t* ws, 
   *pos = pin;
 }
 
+int64_t sort_words(int64_t n, int64_t V) {
+  const SortPlan p = sort_plan(n, V);
+  return p.small ? 2 * n : (4 * n + 1) / 2 * 2 + (int64_t(p.tiles) << p.bits);
+}
+
+template <typename TW, typename TO, int VEC>
+void embed_sum_t(const uint32_t* keys, const uint32_t* pos, int64_t n, const TO* dy, int64_t dys, TW* dw, float* part,
+                 int64_t V, int64_t D, float scale, hipStream_t stream) {
+  const SumPlan s = sum_plan(n, D, VEC);
+  const int64_t sums = ((s.pieces * s.chunks << s.lpr) + 255) / 256, zeros = (V + kZeroRows - 1) / kZeroRows;
+  if (sums + zeros > (int64_t(1) << 31) - 1) throw std::invalid_argument("embedding_grad: too many elements");
+  hipLaunchKernelGGL((k_embed_sum<TW, TO, VEC>), dim3(uint32_t(sums + zeros)), dim3(256), 0, stream, keys, pos,
+                     uint32_t(n), dy, dys, dw, part, V, D, scale, s, uint32_t(sums));
+  if (s.pieces > 1)
+    hipLaunchKernelGGL((k_embed_join<TW, VEC>), dim3(uint32_t(s.pieces * s.chunks)), dim3(256), 0, stream, keys,
+                       uint32_t(n), part, dw, V, D, scale, s);
+  RMM_HIP_CHECK(hipGetLastError());
+}
+
+// 16 bytes of dy a lane where the rows allow it, else pairs, else single elements.
 template <typename TW, typename TO>
-void embed_rows_t(const uint32_t* keys, const uint32_t* pos, int64_t n, const void* dy, int64_t dys, void* dw, int64_t V,
-                  int64_t D, float scale, hipStream_t stream) {
-  constexpr int VEC = 8;
-  const bool wide = D % VEC == 0 && dys % VEC == 0 && vec_aligned<TO, VEC>(dy) && vec_aligned<TW, VEC>(dw);
-  const int lpr = lanes_log2(D, wide ? VEC : 1);
-  const uint32_t blocks = row_blocks(V, lpr, "embedding_grad");
+void embed_sum_any(const uint32_t* keys, const uint32_t* pos, int64_t n, const void* dy, int64_t dys, void* dw,
+                   float* part, int64_t V, int64_t D, float scale, hipStream_t stream) {
+  constexpr int VEC = 16 / sizeof(TO);
   const TO* yp = static_cast<const TO*>(dy);
   TW* wp = static_cast<TW*>(dw);
-  if (wide)
-    hipLaunchKernelGGL((k_embed_rows<TW, TO, VEC>), dim3(blocks), dim3(256), 0, stream, keys, pos, uint32_t(n), yp, dys,
-                       wp, V, D, scale, lpr);
+  if (D % VEC == 0 && dys % VEC == 0 && vec_aligned<TO, VEC>(dy) && vec_aligned<TW, VEC>(dw))
+    embed_sum_t<TW, TO, VEC>(keys, pos, n, yp, dys, wp, part, V, D, scale, stream);
+  else if (D % 2 == 0 && dys % 2 == 0 && vec_aligned<TO, 2>(dy) && vec_aligned<TW, 2>(dw))
+    embed_sum_t<TW, TO, 2>(keys, pos, n, yp, dys, wp, part, V, D, scale, stream);
   else
-    hipLaunchKernelGGL((k_embed_rows<TW, TO, 1>), dim3(blocks), dim3(256), 0, stream, keys, pos, uint32_t(n), yp, dys,
-                       wp, V, D, scale, lpr);
-  RMM_HIP_CHECK(hipGetLastError());
+    embed_sum_t<TW, TO, 1>(keys, pos, n, yp, dys, wp, part, V, D, scale, stream);
 }
 
 }  // namespace
@@ -294,28 +538,30 @@ void embedding_fwd(const void* ids, bool ids64, const void* w, int wtype, int64_
   });
 }
 
-int64_t embedding_grad_workspace(int64_t n, int64_t V) {
-  if (n <= 0) return 0;
-  const SortPlan p = sort_plan(n, V);
-  return (4 * n + (int64_t(p.tiles) << p.bits)) * int64_t(sizeof(uint32_t));
+int64_t embedding_grad_workspace(int64_t n, int64_t V, int64_t D) {
+  if (n <= 0 || D <= 0) return 0;
+  const int64_t pieces = (n + 15) / 16;  // the shortest
+  return (sort_words(n, V) + 3) / 4 * 16 + (pieces > 1 ? 2 * pieces * D * int64_t(sizeof(float)) : 0);
 }
 
 void embedding_grad(const void* ids, bool ids64, const void* dy, int otype, int64_t dystride, void* dw, int wtype,
                     int64_t n, int64_t V, int64_t D, int64_t pad, float scale, void* workspace, hipStream_t stream) {
   if (V <= 0 || D <= 0) return;
   constexpr int64_t kMax = (int64_t(1) << 31) - 1;
-  if (n > kMax || V >= kMax) throw std::invalid_argument("embedding_grad: at most 2^31 - 1 tokens and rows");
+  if (n >= kMax || V >= kMax) throw std::invalid_argument("embedding_grad: fewer than 2^31 - 1 tokens and rows");
   if (n > 0 && workspace == nullptr) throw std::invalid_argument("embedding_grad: no workspace");
   const uint32_t *keys = nullptr, *pos = nullptr;
+  float* part = nullptr;
   if (n > 0) {
     uint32_t* ws = static_cast<uint32_t*>(workspace);
+    part = reinterpret_cast<float*>(ws + (sort_words(n, V) + 3) / 4 * 4);
     if (ids64)
       embed_sort(static_cast<const int64_t*>(ids), n, V, pad, ws, &keys, &pos, stream);
     else
       embed_sort(static_cast<const int32_t*>(ids), n, V, pad, ws, &keys, &pos, stream);
   }
   dispatch_types(wtype, otype, "embedding_grad", [&](auto tw, auto to) {
-    embed_rows_t<decltype(tw), decltype(to)>(keys, pos, n, dy, dystride, dw, V, D, scale, stream);
+    embed_sum_any<decltype(tw), decltype(to)>(keys, pos, n, dy, dystride, dw, part, V, D, scale, stream);
   });
 }
 

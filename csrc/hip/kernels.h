@@ -147,10 +147,10 @@ struct DenseFinalize {
 // K22: embedding lookup out[i] = scale * W[id_i] (zeros for ids outside [0, V)) and its gradient
 // dW[v] = scale * sum of dy[i] over id_i = v, summed in fp32 in the order of i; `pad` (or -1) is a row whose
 // gradient stays zero. W rows are wstride elements apart, dy rows dystride; out and dW are dense. Element types are
-// the codes of vec_types.h. The workspace holds embedding_grad_workspace(n, V) bytes.
+// the codes of vec_types.h. The workspace holds embedding_grad_workspace(n, V, D) bytes, 16-byte aligned.
 void embedding_fwd(const void* ids, bool ids64, const void* w, int wtype, int64_t wstride, void* out, int otype,
                    int64_t n, int64_t V, int64_t D, float scale, hipStream_t stream);
-int64_t embedding_grad_workspace(int64_t n, int64_t V);
+int64_t embedding_grad_workspace(int64_t n, int64_t V, int64_t D);
 void embedding_grad(const void* ids, bool ids64, const void* dy, int otype, int64_t dystride, void* dw, int wtype,
                     int64_t n, int64_t V, int64_t D, int64_t pad, float scale, void* workspace, hipStream_t stream);
 

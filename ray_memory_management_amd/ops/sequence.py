@@ -78,7 +78,7 @@ class _Embedding(torch.autograd.Function):
         n = ids.numel()
         dy = _rows(dy.reshape(n, D))
         dw = torch.empty((V, D), dtype=dtype, device=dy.device)
-        ws = torch.empty(h.embedding_grad_workspace(n, V), dtype=torch.uint8, device=dy.device)
+        ws = torch.empty(h.embedding_grad_workspace(n, V, D), dtype=torch.uint8, device=dy.device)
         with _device(dy):
             h.embedding_grad(ids.data_ptr(), ids.dtype == torch.int64, dy.data_ptr(), _CODE[dy.dtype], dy.stride(0),
                              dw.data_ptr(), _CODE[dtype], n, V, D, padding_idx, scale, ws.data_ptr(), _stream(dy))

@@ -170,7 +170,7 @@ struct ScanArgs {
   const uint8_t* resets = nullptr;             // [B, L], null: none
   const int64_t* lengths = nullptr;            // [B], null: all L
   float* ckpt = nullptr;                       // [B, gated_scan_checkpoints(L, type), D]: written by fwd (null: not), read by bwd
-  void* workspace = nullptr;                   // gated_scan_workspace(B, L, D, type) bytes, 8-byte aligned
+  void* workspace = nullptr;                   // gated_scan_workspace(B, L, D, type) bytes, 8-byte aligned (none: null)
   float* h_last = nullptr;                     // [B, D]
   const float* dh_last = nullptr;              // [B, D], null: zeros
   float* dh0 = nullptr;                        // [B, D], null: not wanted

@@ -421,7 +421,8 @@ int64_t gated_scan_workspace(int64_t B, int64_t L, int64_t D, int type) {
   ScanArgs p;
   p.B = B, p.L = L, p.D = D;
   if (B <= 0 || D <= 0) return 0;
-  return scan_words(p, scan_plan(p, type, 1, "gated_scan")) * int64_t(sizeof(uint64_t)) + 64;
+  const int64_t n = scan_words(p, scan_plan(p, type, 1, "gated_scan"));
+  return n ? n * int64_t(sizeof(uint64_t)) + 64 : 0;
 }
 
 void gated_scan_fwd(const ScanArgs& p, const void* x, const void* g, void* y, int type, hipStream_t stream) {

@@ -7,7 +7,6 @@ graph: nothing synchronises, and what a call keeps for its backward pass belongs
 """
 from __future__ import annotations
 
-import contextlib
 from typing import Optional, Tuple, Union
 
 import torch
@@ -19,16 +18,32 @@ from ray_memory_management_amd._native import require_hip
 __all__ = ["embedding", "Embedding", "dropout", "Dropout", "gated_scan", "gated_scan_step"]
 
 _CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # vec_types.h ElemType
-_NULL = contextlib.nullcontext()
 
 
-def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+def _launch(fn, t: torch.Tensor, *args) -> None:
+    """fn(*args, stream) on the current stream of t's device, with that device the current one. The raw stream handle:
+    building a torch.cuda.Stream takes longer than the launch."""
+    d = t.get_device()
+    if d == torch._C._cuda_getDevice():
+        fn(*args, torch._C._cuda_getCurrentRawStream(d))
+    else:
+        with torch.cuda.device(d):
+            fn(*args, torch._C._cuda_getCurrentRawStream(d))
 
 
-def _device(t: torch.Tensor):
-    """Context in which t's device is the current one (launches go to the current device)."""
-    return _NULL if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _first_order(backward):
+    """A backward pass that cannot be differentiated again says so when it is (only a pass with create_graph runs with
+    gradients enabled, and pays for that bookkeeping)."""
+    checked = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
@@ -43,9 +58,10 @@ def _code(who: str, t: torch.dtype) -> int:
 
 
 def _same_device(who: str, ref: torch.Tensor, **tensors) -> None:
+    dev = ref.device
     for name, t in tensors.items():
-        if t is not None and t.device != ref.device:
-            raise ValueError(f"{who}: {name} is on {t.device}, not on {ref.device}")
+        if t is not None and t.device != dev:
+            raise ValueError(f"{who}: {name} is on {t.device}, not on {dev}")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -54,23 +70,24 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 # ------------------------------------------------------------------------------------------ embedding
+def _embedding_fwd(ids, weight, scale, dtype):
+    V, D = weight.shape
+    w = _rows(weight)
+    out = torch.empty((*ids.shape, D), dtype=dtype, device=weight.device)
+    _launch(require_hip().embedding_fwd, out, ids.data_ptr(), ids.dtype == torch.int64, w.data_ptr(), _CODE[w.dtype],
+            w.stride(0), out.data_ptr(), _CODE[dtype], ids.numel(), V, D, scale)
+    return out
+
+
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx, dtype):
-        h = require_hip()
-        V, D = weight.shape
-        n = ids.numel()
-        w = _rows(weight.detach())
-        out = torch.empty((*ids.shape, D), dtype=dtype, device=weight.device)
-        with _device(weight):
-            h.embedding_fwd(ids.data_ptr(), ids.dtype == torch.int64, w.data_ptr(), _CODE[w.dtype], w.stride(0),
-                            out.data_ptr(), _CODE[dtype], n, V, D, scale, _stream(weight))
         ctx.save_for_backward(ids)
-        ctx.meta = (V, D, scale, padding_idx, weight.dtype)
-        return out
+        ctx.meta = (*weight.shape, scale, padding_idx, weight.dtype)
+        return _embedding_fwd(ids, weight, scale, dtype)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
         V, D, scale, padding_idx, dtype = ctx.meta
@@ -79,9 +96,8 @@ class _Embedding(torch.autograd.Function):
         dy = _rows(dy.reshape(n, D))
         dw = torch.empty((V, D), dtype=dtype, device=dy.device)
         ws = torch.empty(h.embedding_grad_workspace(n, V, D), dtype=torch.uint8, device=dy.device)
-        with _device(dy):
-            h.embedding_grad(ids.data_ptr(), ids.dtype == torch.int64, dy.data_ptr(), _CODE[dy.dtype], dy.stride(0),
-                             dw.data_ptr(), _CODE[dtype], n, V, D, padding_idx, scale, ws.data_ptr(), _stream(dy))
+        _launch(h.embedding_grad, dy, ids.data_ptr(), ids.dtype == torch.int64, dy.data_ptr(), _CODE[dy.dtype],
+                dy.stride(0), dw.data_ptr(), _CODE[dtype], n, V, D, padding_idx, scale, ws.data_ptr())
         return None, dw, None, None, None
 
 
@@ -120,12 +136,15 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
         pad = int(padding_idx) % V
     if not dtype.is_floating_point or not weight.dtype.is_floating_point:
         raise ValueError("embedding: floating-point weight and output types")
-    if weight.device.type != "cuda":
+    if not weight.is_cuda:
         return _embedding_cpu(ids, weight, float(scale), pad, dtype)
     _code("embedding", weight.dtype), _code("embedding", dtype)
     if max(ids.numel(), V) >= 2 ** 31 - 1:
         raise ValueError("embedding: fewer than 2^31 - 1 ids and rows")
-    return _Embedding.apply(ids.contiguous(), weight, float(scale), pad, dtype)
+    ids, scale = ids.contiguous(), float(scale)
+    if not _wants_grad(weight):
+        return _embedding_fwd(ids, weight, scale, dtype)
+    return _Embedding.apply(ids, weight, scale, pad, dtype)
 
 
 class Embedding(nn.Embedding):
@@ -182,34 +201,31 @@ def _dropout_cpu(x, p, seed, offset, residual):
     return (y if residual is None else y + residual.to(y.dtype)).to(x.dtype)
 
 
+def _dropout_run(x, residual, p, seed, offset, ctr, used):
+    x = x.contiguous()
+    out = torch.empty_like(x)
+    if residual is not None:
+        residual = residual.contiguous()
+    _launch(require_hip().dropout, x, x.data_ptr(), _ptr(residual), out.data_ptr(), _CODE[x.dtype], x.numel(), p, seed,
+            offset, _ptr(ctr), _ptr(used))
+    return out
+
+
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, p, seed, offset):
-        xc = x.detach().contiguous()
-        rc = None if residual is None else residual.detach().contiguous()
-        out = torch.empty_like(xc)
-        ctr = offset if isinstance(offset, torch.Tensor) else None
-        used = torch.empty(1, dtype=torch.int64, device=x.device) if ctr is not None else None
-        with _device(x):
-            require_hip().dropout(xc.data_ptr(), _ptr(rc), out.data_ptr(), _CODE[x.dtype], xc.numel(), p, seed,
-                                  0 if ctr is not None else offset, _ptr(ctr), _ptr(used), _stream(x))
+    def forward(ctx, x, residual, p, seed, offset, ctr):
+        used = None if ctr is None else torch.empty(1, dtype=torch.int64, device=x.device)
         ctx.save_for_backward(used)
-        ctx.meta = (p, seed, 0 if ctr is not None else offset)
-        return out
+        ctx.meta = (p, seed, offset)
+        return _dropout_run(x, residual, p, seed, offset, ctr, used)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         (used,) = ctx.saved_tensors
-        p, seed, offset = ctx.meta
-        dx = None
-        if ctx.needs_input_grad[0]:
-            d = dy.contiguous()
-            dx = torch.empty_like(d)
-            with _device(d):
-                require_hip().dropout(d.data_ptr(), 0, dx.data_ptr(), _CODE[d.dtype], d.numel(), p, seed, offset,
-                                      _ptr(used), 0, _stream(d))
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+        need = ctx.needs_input_grad
+        dx = _dropout_run(dy, None, *ctx.meta, used, None) if need[0] else None
+        return dx, dy if need[1] else None, None, None, None, None
 
 
 def dropout(x: torch.Tensor, p: float, seed: int, offset: Union[int, torch.Tensor] = 0,
@@ -229,24 +245,24 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: Union[int, torch.Tenso
         if residual.shape != x.shape or residual.dtype != x.dtype:
             raise ValueError(f"dropout: residual must match x: {tuple(residual.shape)} {residual.dtype} against "
                              f"{tuple(x.shape)} {x.dtype}")
+        _same_device("dropout", x, residual=residual)
+    ctr = None
     if isinstance(offset, torch.Tensor):
         if offset.dtype != torch.int64 or offset.numel() < 1:
             raise ValueError("dropout: an offset tensor holds int64")
         _same_device("dropout", x, offset=offset)
-    else:
-        offset = int(offset) & 0xFFFFFFFFFFFFFFFF
-    _same_device("dropout", x, residual=residual)
+        ctr, offset = offset, 0
     if not x.dtype.is_floating_point:
         raise ValueError(f"dropout: a floating-point tensor, not {x.dtype}")
     if not training:
         return x if residual is None else x + residual
-    seed = int(seed) & 0xFFFFFFFFFFFFFFFF
-    if x.device.type != "cuda":
-        if isinstance(offset, torch.Tensor):
-            offset = int(offset.reshape(-1)[0])
-        return _dropout_cpu(x, float(p), seed, offset, residual)
+    p, seed, offset = float(p), int(seed) & 0xFFFFFFFFFFFFFFFF, int(offset) & 0xFFFFFFFFFFFFFFFF
+    if not x.is_cuda:
+        return _dropout_cpu(x, p, seed, offset if ctr is None else int(ctr.reshape(-1)[0]), residual)
     _code("dropout", x.dtype)
-    return _Dropout.apply(x, residual, float(p), seed, offset)
+    if not _wants_grad(x, residual):
+        return _dropout_run(x, residual, p, seed, offset, ctr, None)
+    return _Dropout.apply(x, residual, p, seed, offset, ctr)
 
 
 class Dropout(nn.Module):
@@ -309,60 +325,70 @@ def _scan_cpu(x, gate, h0, resets, lengths):
     return (torch.stack(ys, dim=1) if L else x.new_zeros((B, 0, D), dtype=st)), h
 
 
+def _gate_place(x, gate, D):
+    """Address and strides of the gates: their own tensor, or the second half of x."""
+    if gate is None:
+        return x.data_ptr() + D * x.element_size(), x.stride(0), x.stride(1)
+    return gate.data_ptr(), gate.stride(0), gate.stride(1)
+
+
 def _scan_workspace(h, B, L, D, x):
-    return torch.empty(h.gated_scan_workspace(B, L, D, _CODE[x.dtype]), dtype=torch.uint8, device=x.device)
+    n = h.gated_scan_workspace(B, L, D, _CODE[x.dtype])
+    return torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+
+
+def _scan_fwd(x, gate, h0, resets, lengths, keep):
+    """(y, h_last, the states kept for a backward pass or None) of rows with consecutive channels."""
+    h = require_hip()
+    B, L, D = x.shape
+    if gate is None:
+        D //= 2
+    dev, code = x.device, _CODE[x.dtype]
+    y = torch.empty((B, L, D), dtype=x.dtype, device=dev)
+    h_last = torch.empty((B, D), dtype=torch.float32, device=dev)
+    ckpt = torch.empty((B, h.gated_scan_checkpoints(L, code), D), dtype=torch.float32, device=dev) if keep else None
+    ws = _scan_workspace(h, B, L, D, x)
+    gp, gsb, gst = _gate_place(x, gate, D)
+    _launch(h.gated_scan_fwd, x, x.data_ptr(), gp, y.data_ptr(), code, (B, L, D), (x.stride(0), x.stride(1), gsb, gst),
+            _ptr(h0), _ptr(resets), _ptr(lengths), _ptr(ckpt), h_last.data_ptr(), _ptr(ws))
+    return y, h_last, ckpt
 
 
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, h0, resets, lengths):
         ctx.set_materialize_grads(False)
-        h = require_hip()
-        x = _rows(x.detach())
-        B, L, D = x.shape
-        if gate is None:
-            D //= 2
-            g, gs, gp = None, (x.stride(0), x.stride(1)), x.data_ptr() + D * x.element_size()
-        else:
-            g = _rows(gate.detach())
-            gs, gp = (g.stride(0), g.stride(1)), g.data_ptr()
-        y = torch.empty((B, L, D), dtype=x.dtype, device=x.device)
-        h_last = torch.empty((B, D), dtype=torch.float32, device=x.device)
-        ckpt = None
-        if any(ctx.needs_input_grad):
-            ckpt = torch.empty((B, h.gated_scan_checkpoints(L, _CODE[x.dtype]), D), dtype=torch.float32, device=x.device)
-        ws = _scan_workspace(h, B, L, D, x)
-        with _device(x):
-            h.gated_scan_fwd(x.data_ptr(), gp, y.data_ptr(), _CODE[x.dtype], (B, L, D),
-                             (x.stride(0), x.stride(1), *gs), _ptr(h0), _ptr(resets), _ptr(lengths), _ptr(ckpt),
-                             h_last.data_ptr(), ws.data_ptr(), _stream(x))
-        ctx.save_for_backward(x, g, resets, lengths, ckpt)
+        x, gate = _rows(x), None if gate is None else _rows(gate)
+        y, h_last, ckpt = _scan_fwd(x, gate, h0, resets, lengths, True)
+        ctx.save_for_backward(x, gate, resets, lengths, ckpt)
         return y, h_last
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy, dh):
-        x, g, resets, lengths, ckpt = ctx.saved_tensors
+        x, gate, resets, lengths, ckpt = ctx.saved_tensors
         h = require_hip()
         B, L, D = x.shape
-        if g is None:
+        dev = x.device
+        dx, dg = torch.empty((B, L, D), dtype=x.dtype, device=dev), None
+        ds = (L * D, D)
+        if gate is None:
             D //= 2
-            gs, gp = (x.stride(0), x.stride(1)), x.data_ptr() + D * x.element_size()
-            dx, dg, ds = torch.empty((B, L, 2 * D), dtype=x.dtype, device=x.device), None, (L * 2 * D, 2 * D)
             dgp = dx.data_ptr() + D * x.element_size()
         else:
-            gs, gp = (g.stride(0), g.stride(1)), g.data_ptr()
-            dx, dg = (torch.empty((B, L, D), dtype=x.dtype, device=x.device) for _ in range(2))
-            ds, dgp = (L * D, D), dg.data_ptr()
-        dh0 = torch.empty((B, D), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
-        dy = None if dy is None else _rows(dy)
+            dg = torch.empty((B, L, D), dtype=x.dtype, device=dev)
+            dgp = dg.data_ptr()
+        dh0 = torch.empty((B, D), dtype=torch.float32, device=dev) if ctx.needs_input_grad[2] else None
+        ys = (0, 0)
+        if dy is not None:
+            dy = _rows(dy)
+            ys = (dy.stride(0), dy.stride(1))
         dh = None if dh is None else dh.contiguous()
-        ys = (0, 0) if dy is None else (dy.stride(0), dy.stride(1))
         ws = _scan_workspace(h, B, L, D, x)
-        with _device(x):
-            h.gated_scan_bwd(x.data_ptr(), gp, _ptr(dy), dx.data_ptr(), dgp, _CODE[x.dtype], (B, L, D),
-                             (x.stride(0), x.stride(1), *gs, *ys, *ds), _ptr(resets), _ptr(lengths), _ptr(ckpt),
-                             _ptr(dh), _ptr(dh0), ws.data_ptr(), _stream(x))
+        gp, gsb, gst = _gate_place(x, gate, D)
+        _launch(h.gated_scan_bwd, x, x.data_ptr(), gp, _ptr(dy), dx.data_ptr(), dgp, _CODE[x.dtype], (B, L, D),
+                (x.stride(0), x.stride(1), gsb, gst, *ys, *ds), _ptr(resets), _ptr(lengths), _ptr(ckpt), _ptr(dh),
+                _ptr(dh0), _ptr(ws))
         return dx, dg, dh0, None, None
 
 
@@ -413,7 +439,7 @@ def gated_scan(x: torch.Tensor, gate: Optional[torch.Tensor] = None, h0: Optiona
                                 or lengths.dtype.is_complex or lengths.dtype == torch.bool):
         raise ValueError(f"gated_scan: lengths must be {B} integers, not {tuple(lengths.shape)} {lengths.dtype}")
     resets = _flags("gated_scan", resets, (B, L))
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         if gate is None:
             x, gate = x[..., :D], x[..., D:]
         h0 = x.new_zeros((B, D), dtype=torch.promote_types(x.dtype, torch.float32)) if h0 is None else h0
@@ -422,7 +448,10 @@ def gated_scan(x: torch.Tensor, gate: Optional[torch.Tensor] = None, h0: Optiona
     _code("gated_scan", x.dtype)
     h0 = None if h0 is None else h0.to(torch.float32).contiguous()
     lengths = None if lengths is None else lengths.to(torch.int64).contiguous()
-    return _GatedScan.apply(x, gate, h0, None if resets is None else resets.view(torch.uint8), lengths)
+    resets = None if resets is None else resets.view(torch.uint8)
+    if not _wants_grad(x, gate, h0):
+        return _scan_fwd(_rows(x), None if gate is None else _rows(gate), h0, resets, lengths, False)[:2]
+    return _GatedScan.apply(x, gate, h0, resets, lengths)
 
 
 def gated_scan_step(x: torch.Tensor, gate: Optional[torch.Tensor], state: torch.Tensor,
@@ -438,14 +467,14 @@ def gated_scan_step(x: torch.Tensor, gate: Optional[torch.Tensor], state: torch.
     for name, t in (("state", state), ("out", out)):
         if t is not None and (tuple(t.shape) != (B, D) or t.dtype != torch.float32 or not t.is_contiguous()):
             raise ValueError(f"gated_scan_step: {name} must be {(B, D)}, fp32 and contiguous")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, state)):
+    if _wants_grad(x, gate, state):
         raise ValueError("gated_scan_step is not differentiable: call gated_scan with L = 1, or under torch.no_grad()")
     if out is not None:
         delta = abs(out.data_ptr() - state.data_ptr())
         if 0 < delta < state.numel() * 4:
             raise ValueError("gated_scan_step: out overlaps state without being it")
     resets = _flags("gated_scan_step", resets, (B,))
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         if gate is None:
             x, gate = x[..., :D], x[..., D:]
         prev = state if resets is None else torch.where(resets.unsqueeze(-1), torch.zeros(()), state)
@@ -461,7 +490,6 @@ def gated_scan_step(x: torch.Tensor, gate: Optional[torch.Tensor], state: torch.
         gp, gs = gate.data_ptr(), gate.stride(0)
     out = torch.empty_like(state) if out is None else out
     y = torch.empty((B, D), dtype=x.dtype, device=x.device)
-    with _device(x):
-        require_hip().gated_scan_step(x.data_ptr(), x.stride(0), gp, gs, _ptr(resets), state.data_ptr(),
-                                      out.data_ptr(), y.data_ptr(), code, B, D, _stream(x))
+    _launch(require_hip().gated_scan_step, x, x.data_ptr(), x.stride(0), gp, gs, _ptr(resets), state.data_ptr(),
+            out.data_ptr(), y.data_ptr(), code, B, D)
     return y, out

@@ -3,6 +3,7 @@
 * ``_store``  — shared-memory object store (C++17, g++)
 * ``_sched``  — scheduler core: resource sets, policies, dependency-gated queue (C++17, g++)
 * ``_envs``   — native env cores (synthetic Atari vector env) for CPU rollout workers (C++17, g++)
+* ``_seq``    — sequence kernels (embedding, dropout, gated scan) as torch operators (HIP + libtorch, hipcc)
 * ``_hip``    — CDNA4 kernels + HBM GPU object store + native hybrid rollout loop (HIP, hipcc --offload-arch=gfx950)
 
 Usage: ``python build_native.py [--force] [--only NAME]``. Rebuilds an extension only when a
@@ -60,6 +61,10 @@ def extensions():
              common, ["-lpthread"], ["csrc/sched/scheduler.h"]),
         _ext("_envs", ["csrc/rl/envs_py.cc"], "g++", common, [], ["csrc/rl/synth_env.h"]),
     ]
+    # no packed fp32 instructions (v_pk_{add,mul,fma}_f32): some of their forms give wrong results now and then on
+    # this hardware. The host pass does not know the feature and says so.
+    hip_flags = [f"--offload-arch={ARCH}", "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang",
+                 "-packed-fp32-ops"]
     tl = _torch_lib()
     hip_ld = ["-lpthread"]
     # Link against the HIP runtime torch ships with (same soname as /opt/rocm's) so one runtime
@@ -67,17 +72,25 @@ def extensions():
     if tl:
         hip_ld = [f"-L{tl}", f"-Wl,-rpath,{tl}", "-lamdhip64"] + hip_ld
     exts.append(
-        _ext("_hip", ["csrc/hip/kernels.hip", "csrc/hip/rl_kernels.hip", "csrc/hip/conv_kernels.hip", "csrc/hip/dense_kernels.hip", "csrc/hip/x3_kernels.hip", "csrc/hip/shuffle_kernels.hip", "csrc/hip/ingest_kernels.hip", "csrc/hip/vtrace_kernels.hip", "csrc/hip/embedding_kernels.hip", "csrc/hip/dropout_kernels.hip", "csrc/hip/scan_kernels.hip", "csrc/hip/gpu_store.hip", "csrc/hip/peer_allreduce.hip", "csrc/hip/rollout_server.hip", "csrc/hip/rccl_comm.cc", "csrc/hip/rollout_loop.cc", "csrc/hip/hip_py.cc",
+        _ext("_hip", ["csrc/hip/kernels.hip", "csrc/hip/rl_kernels.hip", "csrc/hip/conv_kernels.hip", "csrc/hip/dense_kernels.hip", "csrc/hip/x3_kernels.hip", "csrc/hip/shuffle_kernels.hip", "csrc/hip/ingest_kernels.hip", "csrc/hip/vtrace_kernels.hip", "csrc/hip/gpu_store.hip", "csrc/hip/peer_allreduce.hip", "csrc/hip/rollout_server.hip", "csrc/hip/rccl_comm.cc", "csrc/hip/rollout_loop.cc", "csrc/hip/hip_py.cc",
               "csrc/store/shm_store.cc"], HIPCC,
-             # no packed fp32 instructions (v_pk_{add,mul,fma}_f32): some of their forms give wrong results
-             # now and then on this hardware. The host pass does not know the feature and says so.
-             common + [f"--offload-arch={ARCH}", "-munsafe-fp-atomics", "-Wno-unused-result",
-                       "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+             common + hip_flags + ["-munsafe-fp-atomics"]
              # RMM_X3_PROBE=1: the x3 kernels' phase timestamps (benchmarks/x3_phase_probe.py; build with --force)
              + (["-DRMM_X3_PROBE"] if os.environ.get("RMM_X3_PROBE") == "1" else []),
              hip_ld, ["csrc/hip/kernels.h", "csrc/hip/gpu_store.h", "csrc/hip/rccl_comm.h", "csrc/hip/peer_allreduce.h", "csrc/hip/common.h", "csrc/store/shm_store.h",
                      "csrc/hip/rollout_loop.h", "csrc/rl/synth_env.h", "csrc/hip/trunk_device.h",
-                     "csrc/hip/dense_device.h", "csrc/hip/adam_device.h", "csrc/hip/x3_device.h", "csrc/hip/vec_types.h"]))
+                     "csrc/hip/dense_device.h", "csrc/hip/adam_device.h", "csrc/hip/x3_device.h"]))
+    if tl:
+        # torch's own pybind11 goes first: its tensor casters are built against it
+        ti = os.path.join(os.path.dirname(tl), "include")
+        torch_inc = [f"-I{ti}", f"-I{os.path.join(ti, 'torch', 'csrc', 'api', 'include')}"]
+        exts.append(
+            _ext("_seq", ["csrc/hip/embedding_kernels.hip", "csrc/hip/dropout_kernels.hip", "csrc/hip/scan_kernels.hip",
+                          "csrc/hip/seq_torch.cc"], HIPCC,
+                 torch_inc + common + hip_flags + ["-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__=1", "-DTORCH_EXTENSION_NAME=_seq",
+                                                   "-DTORCH_API_INCLUDE_EXTENSION_H"],
+                 ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"] + hip_ld,
+                 ["csrc/hip/kernels.h", "csrc/hip/common.h", "csrc/hip/vec_types.h"]))
     return exts
 
 

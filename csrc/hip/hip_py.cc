@@ -4,7 +4,6 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
-#include <array>
 #include <cstring>
 #include <memory>
 
@@ -296,52 +295,6 @@ PYBIND11_MODULE(_hip, m) {
     vtrace(P<const float>(blogp), P<const float>(tlogp), P<const float>(rew), P<const float>(val),
            P<const float>(done), P<const float>(boot), T, B, gamma, clip_rho, clip_pg_rho, lam, P<float>(vs),
            P<float>(pg), S(stream));
-  });
-  m.def("embedding_fwd", [](uint64_t ids, bool ids64, uint64_t w, int wtype, int64_t wstride, uint64_t out, int otype,
-                            int64_t n, int64_t V, int64_t D, float scale, uint64_t stream) {
-    embedding_fwd(P<const void>(ids), ids64, P<const void>(w), wtype, wstride, P<void>(out), otype, n, V, D, scale,
-                  S(stream));
-  });
-  m.def("embedding_grad_workspace", &embedding_grad_workspace);
-  m.def("embedding_grad", [](uint64_t ids, bool ids64, uint64_t dy, int otype, int64_t dystride, uint64_t dw, int wtype,
-                             int64_t n, int64_t V, int64_t D, int64_t pad, float scale, uint64_t ws, uint64_t stream) {
-    embedding_grad(P<const void>(ids), ids64, P<const void>(dy), otype, dystride, P<void>(dw), wtype, n, V, D, pad,
-                   scale, P<void>(ws), S(stream));
-  });
-  m.def("dropout", [](uint64_t x, uint64_t res, uint64_t out, int type, int64_t n, double p, uint64_t seed,
-                      uint64_t offset, uint64_t ctr, uint64_t used, uint64_t stream) {
-    dropout(P<const void>(x), P<const void>(res), P<void>(out), type, n, p, seed, offset, P<const int64_t>(ctr),
-            P<int64_t>(used), S(stream));
-  });
-  m.def("gated_scan_checkpoints", &gated_scan_checkpoints);
-  m.def("gated_scan_workspace", &gated_scan_workspace);
-  // dims = B, L, D; strides = x (sequence, step), gate, [dy, gradients]
-  m.def("gated_scan_fwd", [](uint64_t x, uint64_t g, uint64_t y, int type, std::array<int64_t, 3> dims,
-                             std::array<int64_t, 4> st, uint64_t h0, uint64_t resets, uint64_t lengths, uint64_t ckpt,
-                             uint64_t h_last, uint64_t ws, uint64_t stream) {
-    ScanArgs p;
-    p.B = dims[0], p.L = dims[1], p.D = dims[2];
-    p.xsb = st[0], p.xst = st[1], p.gsb = st[2], p.gst = st[3];
-    p.h0 = P<const float>(h0), p.resets = P<const uint8_t>(resets), p.lengths = P<const int64_t>(lengths);
-    p.ckpt = P<float>(ckpt), p.h_last = P<float>(h_last), p.workspace = P<void>(ws);
-    gated_scan_fwd(p, P<const void>(x), P<const void>(g), P<void>(y), type, S(stream));
-  });
-  m.def("gated_scan_bwd", [](uint64_t x, uint64_t g, uint64_t dy, uint64_t dx, uint64_t dg, int type,
-                             std::array<int64_t, 3> dims, std::array<int64_t, 8> st, uint64_t resets, uint64_t lengths,
-                             uint64_t ckpt, uint64_t dh_last, uint64_t dh0, uint64_t ws, uint64_t stream) {
-    ScanArgs p;
-    p.B = dims[0], p.L = dims[1], p.D = dims[2];
-    p.xsb = st[0], p.xst = st[1], p.gsb = st[2], p.gst = st[3];
-    p.ysb = st[4], p.yst = st[5], p.dsb = st[6], p.dst = st[7];
-    p.resets = P<const uint8_t>(resets), p.lengths = P<const int64_t>(lengths);
-    p.ckpt = P<float>(ckpt), p.dh_last = P<const float>(dh_last), p.dh0 = P<float>(dh0);
-    p.workspace = P<void>(ws);
-    gated_scan_bwd(p, P<const void>(x), P<const void>(g), P<const void>(dy), P<void>(dx), P<void>(dg), type, S(stream));
-  });
-  m.def("gated_scan_step", [](uint64_t x, int64_t xs, uint64_t g, int64_t gs, uint64_t resets, uint64_t h, uint64_t out,
-                              uint64_t y, int type, int64_t B, int64_t D, uint64_t stream) {
-    gated_scan_step(P<const void>(x), xs, P<const void>(g), gs, P<const uint8_t>(resets), P<const float>(h),
-                    P<float>(out), P<void>(y), type, B, D, S(stream));
   });
   m.def("ingest_block_bytes",[] { return int(sizeof(IngestBlock)); });
   m.def("standardize_col", [](uint64_t cols, int64_t N, int C, int col, uint64_t stats, uint64_t stream) {

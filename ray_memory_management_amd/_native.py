@@ -1,8 +1,8 @@
 """Loader for the in-tree native extensions (built by ``build_native.py``).
 
-``_store`` and ``_sched`` are required everywhere. ``_hip`` is imported lazily (after torch, so
-the process uses ONE HIP runtime) and is REQUIRED whenever a GPU is visible: on a GPU box a
-missing/broken ``_hip`` raises rather than silently falling back to eager PyTorch.
+``_store`` and ``_sched`` are required everywhere. ``_hip`` and ``_seq`` are imported lazily (after torch, so
+the process uses ONE HIP runtime) and are REQUIRED for GPU tensors: a missing/broken extension raises rather
+than silently falling back to eager PyTorch.
 """
 from __future__ import annotations
 
@@ -79,3 +79,21 @@ def require_hip():
             f"ray_memory_management_amd: the native HIP extension (_hip) is required for GPU ops but failed "
             f"to load: {_hip_err!r}. Run `python build_native.py`.")
     return h
+
+
+_seq = None
+
+
+def require_seq():
+    """The sequence operators (``_seq``); raises where they cannot be loaded."""
+    global _seq
+    if _seq is None:
+        try:
+            import torch  # noqa: F401  (its libraries first)
+
+            _seq = load("_seq")
+        except Exception as e:
+            raise RuntimeError(
+                f"ray_memory_management_amd: the native sequence extension (_seq) is required for GPU ops but failed "
+                f"to load: {e!r}. Run `python build_native.py`.") from e
+    return _seq

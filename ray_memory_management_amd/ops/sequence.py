@@ -1,5 +1,6 @@
 """Operators of token and sequence models: embedding with a sorted gradient, counter-based dropout and the gated
-linear recurrence (kernels K22-K24 in ``csrc/hip/{embedding,dropout,scan}_kernels.hip``).
+linear recurrence (kernels K22-K24 in ``csrc/hip/{embedding,dropout,scan}_kernels.hip``, their torch operators with
+autograd in ``csrc/hip/seq_torch.cc``).
 
 CUDA(ROCm) tensors run the HIP kernels on the current stream of their device; CPU tensors the same formulas in torch.
 fp32, bf16 and fp16 are taken on the GPU; sums and states are held in fp32. Everything here can be captured into a
@@ -13,41 +14,11 @@ import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
-from ray_memory_management_amd._native import require_hip
+from ray_memory_management_amd._native import require_seq
 
 __all__ = ["embedding", "Embedding", "dropout", "Dropout", "gated_scan", "gated_scan_step"]
 
-_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # vec_types.h ElemType
-
-
-def _launch(fn, t: torch.Tensor, *args) -> None:
-    """fn(*args, stream) on the current stream of t's device, with that device the current one. The raw stream handle:
-    building a torch.cuda.Stream takes longer than the launch."""
-    d = t.get_device()
-    if d == torch._C._cuda_getDevice():
-        fn(*args, torch._C._cuda_getCurrentRawStream(d))
-    else:
-        with torch.cuda.device(d):
-            fn(*args, torch._C._cuda_getCurrentRawStream(d))
-
-
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _first_order(backward):
-    """A backward pass that cannot be differentiated again says so when it is (only a pass with create_graph runs with
-    gradients enabled, and pays for that bookkeeping)."""
-    checked = once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-
-    return run
-
-
-def _ptr(t: Optional[torch.Tensor]) -> int:
-    return 0 if t is None else t.data_ptr()
+_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # the type codes of the kernels
 
 
 def _code(who: str, t: torch.dtype) -> int:
@@ -64,43 +35,7 @@ def _same_device(who: str, ref: torch.Tensor, **tensors) -> None:
             raise ValueError(f"{who}: {name} is on {t.device}, not on {dev}")
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t with consecutive elements in its last dimension."""
-    return t if t.stride(-1) == 1 else t.contiguous()
-
-
 # ------------------------------------------------------------------------------------------ embedding
-def _embedding_fwd(ids, weight, scale, dtype):
-    V, D = weight.shape
-    w = _rows(weight)
-    out = torch.empty((*ids.shape, D), dtype=dtype, device=weight.device)
-    _launch(require_hip().embedding_fwd, out, ids.data_ptr(), ids.dtype == torch.int64, w.data_ptr(), _CODE[w.dtype],
-            w.stride(0), out.data_ptr(), _CODE[dtype], ids.numel(), V, D, scale)
-    return out
-
-
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ids, weight, scale, padding_idx, dtype):
-        ctx.save_for_backward(ids)
-        ctx.meta = (*weight.shape, scale, padding_idx, weight.dtype)
-        return _embedding_fwd(ids, weight, scale, dtype)
-
-    @staticmethod
-    @_first_order
-    def backward(ctx, dy):
-        (ids,) = ctx.saved_tensors
-        V, D, scale, padding_idx, dtype = ctx.meta
-        h = require_hip()
-        n = ids.numel()
-        dy = _rows(dy.reshape(n, D))
-        dw = torch.empty((V, D), dtype=dtype, device=dy.device)
-        ws = torch.empty(h.embedding_grad_workspace(n, V, D), dtype=torch.uint8, device=dy.device)
-        _launch(h.embedding_grad, dy, ids.data_ptr(), ids.dtype == torch.int64, dy.data_ptr(), _CODE[dy.dtype],
-                dy.stride(0), dw.data_ptr(), _CODE[dtype], n, V, D, padding_idx, scale, ws.data_ptr())
-        return None, dw, None, None, None
-
-
 def _embedding_cpu(ids, weight, scale, padding_idx, dtype):
     ids = ids.long()
     ok = (ids >= 0) & (ids < weight.shape[0])
@@ -141,10 +76,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
     _code("embedding", weight.dtype), _code("embedding", dtype)
     if max(ids.numel(), V) >= 2 ** 31 - 1:
         raise ValueError("embedding: fewer than 2^31 - 1 ids and rows")
-    ids, scale = ids.contiguous(), float(scale)
-    if not _wants_grad(weight):
-        return _embedding_fwd(ids, weight, scale, dtype)
-    return _Embedding.apply(ids, weight, scale, pad, dtype)
+    return require_seq().embedding(ids, weight, scale, pad, _CODE[dtype])
 
 
 class Embedding(nn.Embedding):
@@ -201,33 +133,6 @@ def _dropout_cpu(x, p, seed, offset, residual):
     return (y if residual is None else y + residual.to(y.dtype)).to(x.dtype)
 
 
-def _dropout_run(x, residual, p, seed, offset, ctr, used):
-    x = x.contiguous()
-    out = torch.empty_like(x)
-    if residual is not None:
-        residual = residual.contiguous()
-    _launch(require_hip().dropout, x, x.data_ptr(), _ptr(residual), out.data_ptr(), _CODE[x.dtype], x.numel(), p, seed,
-            offset, _ptr(ctr), _ptr(used))
-    return out
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, p, seed, offset, ctr):
-        used = None if ctr is None else torch.empty(1, dtype=torch.int64, device=x.device)
-        ctx.save_for_backward(used)
-        ctx.meta = (p, seed, offset)
-        return _dropout_run(x, residual, p, seed, offset, ctr, used)
-
-    @staticmethod
-    @_first_order
-    def backward(ctx, dy):
-        (used,) = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx = _dropout_run(dy, None, *ctx.meta, used, None) if need[0] else None
-        return dx, dy if need[1] else None, None, None, None, None
-
-
 def dropout(x: torch.Tensor, p: float, seed: int, offset: Union[int, torch.Tensor] = 0,
             residual: Optional[torch.Tensor] = None, training: bool = True) -> torch.Tensor:
     """``residual + dropout(x)`` whose mask is a function of (seed, offset, element index) and never stored.
@@ -260,9 +165,7 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: Union[int, torch.Tenso
     if not x.is_cuda:
         return _dropout_cpu(x, p, seed, offset if ctr is None else int(ctr.reshape(-1)[0]), residual)
     _code("dropout", x.dtype)
-    if not _wants_grad(x, residual):
-        return _dropout_run(x, residual, p, seed, offset, ctr, None)
-    return _Dropout.apply(x, residual, p, seed, offset, ctr)
+    return require_seq().dropout(x, residual, p, seed, offset, ctr)
 
 
 class Dropout(nn.Module):
@@ -318,78 +221,11 @@ def _scan_cpu(x, gate, h0, resets, lengths):
     z, a = _Gate.apply(gate)
     ys = []
     for t in range(L):
-        prev = h if resets is None else torch.where(resets[:, t, None], torch.zeros((), dtype=st), h)
+        prev = h if resets is None else torch.where((resets != 0)[:, t, None], torch.zeros((), dtype=st), h)
         new = a[:, t] * prev + z[:, t] * x[:, t]
         h = new if live is None else torch.where(live[:, t], new, h)
         ys.append(new if live is None else torch.where(live[:, t], new, torch.zeros((), dtype=new.dtype)))
     return (torch.stack(ys, dim=1) if L else x.new_zeros((B, 0, D), dtype=st)), h
-
-
-def _gate_place(x, gate, D):
-    """Address and strides of the gates: their own tensor, or the second half of x."""
-    if gate is None:
-        return x.data_ptr() + D * x.element_size(), x.stride(0), x.stride(1)
-    return gate.data_ptr(), gate.stride(0), gate.stride(1)
-
-
-def _scan_workspace(h, B, L, D, x):
-    n = h.gated_scan_workspace(B, L, D, _CODE[x.dtype])
-    return torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-
-
-def _scan_fwd(x, gate, h0, resets, lengths, keep):
-    """(y, h_last, the states kept for a backward pass or None) of rows with consecutive channels."""
-    h = require_hip()
-    B, L, D = x.shape
-    if gate is None:
-        D //= 2
-    dev, code = x.device, _CODE[x.dtype]
-    y = torch.empty((B, L, D), dtype=x.dtype, device=dev)
-    h_last = torch.empty((B, D), dtype=torch.float32, device=dev)
-    ckpt = torch.empty((B, h.gated_scan_checkpoints(L, code), D), dtype=torch.float32, device=dev) if keep else None
-    ws = _scan_workspace(h, B, L, D, x)
-    gp, gsb, gst = _gate_place(x, gate, D)
-    _launch(h.gated_scan_fwd, x, x.data_ptr(), gp, y.data_ptr(), code, (B, L, D), (x.stride(0), x.stride(1), gsb, gst),
-            _ptr(h0), _ptr(resets), _ptr(lengths), _ptr(ckpt), h_last.data_ptr(), _ptr(ws))
-    return y, h_last, ckpt
-
-
-class _GatedScan(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gate, h0, resets, lengths):
-        ctx.set_materialize_grads(False)
-        x, gate = _rows(x), None if gate is None else _rows(gate)
-        y, h_last, ckpt = _scan_fwd(x, gate, h0, resets, lengths, True)
-        ctx.save_for_backward(x, gate, resets, lengths, ckpt)
-        return y, h_last
-
-    @staticmethod
-    @_first_order
-    def backward(ctx, dy, dh):
-        x, gate, resets, lengths, ckpt = ctx.saved_tensors
-        h = require_hip()
-        B, L, D = x.shape
-        dev = x.device
-        dx, dg = torch.empty((B, L, D), dtype=x.dtype, device=dev), None
-        ds = (L * D, D)
-        if gate is None:
-            D //= 2
-            dgp = dx.data_ptr() + D * x.element_size()
-        else:
-            dg = torch.empty((B, L, D), dtype=x.dtype, device=dev)
-            dgp = dg.data_ptr()
-        dh0 = torch.empty((B, D), dtype=torch.float32, device=dev) if ctx.needs_input_grad[2] else None
-        ys = (0, 0)
-        if dy is not None:
-            dy = _rows(dy)
-            ys = (dy.stride(0), dy.stride(1))
-        dh = None if dh is None else dh.contiguous()
-        ws = _scan_workspace(h, B, L, D, x)
-        gp, gsb, gst = _gate_place(x, gate, D)
-        _launch(h.gated_scan_bwd, x, x.data_ptr(), gp, _ptr(dy), dx.data_ptr(), dgp, _CODE[x.dtype], (B, L, D),
-                (x.stride(0), x.stride(1), gsb, gst, *ys, *ds), _ptr(resets), _ptr(lengths), _ptr(ckpt), _ptr(dh),
-                _ptr(dh0), _ptr(ws))
-        return dx, dg, dh0, None, None
 
 
 def _scan_parts(who, x, gate):
@@ -406,15 +242,6 @@ def _scan_parts(who, x, gate):
     if gate.shape != x.shape or gate.dtype != x.dtype:
         raise ValueError(f"{who}: gate must match x: {tuple(gate.shape)} {gate.dtype} against {tuple(x.shape)} {x.dtype}")
     return x.shape[-1]
-
-
-def _flags(who, resets, shape):
-    if resets is None:
-        return None
-    if tuple(resets.shape) != tuple(shape):
-        raise ValueError(f"{who}: resets must be {tuple(shape)}, not {tuple(resets.shape)}")
-    resets = resets if resets.dtype == torch.bool else resets != 0
-    return resets.contiguous()
 
 
 def gated_scan(x: torch.Tensor, gate: Optional[torch.Tensor] = None, h0: Optional[torch.Tensor] = None,
@@ -438,7 +265,8 @@ def gated_scan(x: torch.Tensor, gate: Optional[torch.Tensor] = None, h0: Optiona
     if lengths is not None and (tuple(lengths.shape) != (B,) or lengths.dtype.is_floating_point
                                 or lengths.dtype.is_complex or lengths.dtype == torch.bool):
         raise ValueError(f"gated_scan: lengths must be {B} integers, not {tuple(lengths.shape)} {lengths.dtype}")
-    resets = _flags("gated_scan", resets, (B, L))
+    if resets is not None and tuple(resets.shape) != (B, L):
+        raise ValueError(f"gated_scan: resets must be {(B, L)}, not {tuple(resets.shape)}")
     if not x.is_cuda:
         if gate is None:
             x, gate = x[..., :D], x[..., D:]
@@ -446,12 +274,7 @@ def gated_scan(x: torch.Tensor, gate: Optional[torch.Tensor] = None, h0: Optiona
         y, h = _scan_cpu(x, gate, h0, resets, lengths)
         return y.to(x.dtype), h.to(torch.promote_types(x.dtype, torch.float32))
     _code("gated_scan", x.dtype)
-    h0 = None if h0 is None else h0.to(torch.float32).contiguous()
-    lengths = None if lengths is None else lengths.to(torch.int64).contiguous()
-    resets = None if resets is None else resets.view(torch.uint8)
-    if not _wants_grad(x, gate, h0):
-        return _scan_fwd(_rows(x), None if gate is None else _rows(gate), h0, resets, lengths, False)[:2]
-    return _GatedScan.apply(x, gate, h0, resets, lengths)
+    return require_seq().gated_scan(x, gate, h0, resets, lengths)
 
 
 def gated_scan_step(x: torch.Tensor, gate: Optional[torch.Tensor], state: torch.Tensor,
@@ -467,29 +290,20 @@ def gated_scan_step(x: torch.Tensor, gate: Optional[torch.Tensor], state: torch.
     for name, t in (("state", state), ("out", out)):
         if t is not None and (tuple(t.shape) != (B, D) or t.dtype != torch.float32 or not t.is_contiguous()):
             raise ValueError(f"gated_scan_step: {name} must be {(B, D)}, fp32 and contiguous")
-    if _wants_grad(x, gate, state):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, state)):
         raise ValueError("gated_scan_step is not differentiable: call gated_scan with L = 1, or under torch.no_grad()")
     if out is not None:
         delta = abs(out.data_ptr() - state.data_ptr())
         if 0 < delta < state.numel() * 4:
             raise ValueError("gated_scan_step: out overlaps state without being it")
-    resets = _flags("gated_scan_step", resets, (B,))
+    if resets is not None and tuple(resets.shape) != (B,):
+        raise ValueError(f"gated_scan_step: resets must be {(B,)}, not {tuple(resets.shape)}")
     if not x.is_cuda:
         if gate is None:
             x, gate = x[..., :D], x[..., D:]
-        prev = state if resets is None else torch.where(resets.unsqueeze(-1), torch.zeros(()), state)
+        prev = state if resets is None else torch.where((resets != 0).unsqueeze(-1), torch.zeros(()), state)
         h = torch.sigmoid(-gate.float()) * prev + torch.sigmoid(gate.float()) * x.float()
         out = h if out is None else out.copy_(h)
         return out.to(x.dtype, copy=True), out
-    code = _code("gated_scan_step", x.dtype)
-    x = _rows(x)
-    if gate is None:
-        gp, gs = x.data_ptr() + D * x.element_size(), x.stride(0)
-    else:
-        gate = _rows(gate)
-        gp, gs = gate.data_ptr(), gate.stride(0)
-    out = torch.empty_like(state) if out is None else out
-    y = torch.empty((B, D), dtype=x.dtype, device=x.device)
-    _launch(require_hip().gated_scan_step, x, x.data_ptr(), x.stride(0), gp, gs, _ptr(resets), state.data_ptr(),
-            out.data_ptr(), y.data_ptr(), code, B, D)
-    return y, out
+    _code("gated_scan_step", x.dtype)
+    return require_seq().gated_scan_step(x, gate, state, resets, out)

@@ -20,8 +20,9 @@
 // rows. So x, g (and dy) cross the memory bus once for any L, and few channels still fill the card.
 //
 // Waiting. A published word is one 64-bit atomic (A, H) that carries its own readiness in A: all ones before it is
-// written, -1 for a finished state, else in [0, 1]. Workgroups take their place from a ticket counter, and wait only for
-// lower tickets, whose workgroups therefore run already: by induction over the tickets every wait ends.
+// written, -1 for a finished state, else in [0, 1]. The workgroups of a chain (one sequence's 64 VEC channels) take their
+// segments from the chain's ticket counter, and wait only for lower tickets of that counter, whose workgroups therefore
+// run already: by induction over the tickets every wait ends.
 //
 // A = 0 stands for a reset alone: what is before it is dropped, not multiplied by zero (it may be infinite or NaN).
 // Products that underflow are held at the smallest denormal instead, so an infinite state stays infinite.
@@ -86,9 +87,13 @@ __device__ __forceinline__ void publish(uint64_t* p, uint64_t v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-__global__ __launch_bounds__(256) void k_scan_init(uint64_t* __restrict__ words, int64_t n, uint32_t* __restrict__ ticket) {
-  if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) words[i] = ~0ull;
+constexpr int kTicketPitch = 32;  // counters a cache line apart
+
+__global__ __launch_bounds__(256) void k_scan_init(uint64_t* __restrict__ words, int64_t n,
+                                                   uint32_t* __restrict__ tickets, int64_t chains) {
+  const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x, step = int64_t(gridDim.x) * 256;
+  for (int64_t i = at; i < n; i += step) words[i] = ~0ull;
+  for (int64_t i = at; i < chains; i += step) tickets[i * kTicketPitch] = 0;
 }
 
 // States that reach segment `seg` (> 0) of VEC neighbouring chains whose words lie `stride` apart. kLook words of each are
@@ -141,18 +146,18 @@ struct ScanPlace {
   int wave, lane, waves;
 };
 
-// Which (sequence, channels, segment) this workgroup has. Consecutive tickets are different chains, so a chain's
+// Which (sequence, channels, segment) this workgroup has. Neighbouring workgroups are of different chains, so a chain's
 // segments start as far apart as the number of chains allows.
 template <int VEC>
-__device__ __forceinline__ ScanPlace scan_place(const ScanArgs& p, uint32_t* __restrict__ ticket, uint32_t* shared) {
-  uint32_t id = blockIdx.x;
-  if (ticket != nullptr) {
-    if (threadIdx.x == 0) *shared = atomicAdd(ticket, 1u);
-    __syncthreads();
-    id = __builtin_amdgcn_readfirstlane(*shared);
-  }
+__device__ __forceinline__ ScanPlace scan_place(const ScanArgs& p, uint32_t* __restrict__ tickets, uint32_t* shared) {
   const uint32_t tiles = uint32_t((p.D + kWave * VEC - 1) / (kWave * VEC)), chains = uint32_t(p.B) * tiles;
-  const uint32_t seg = id / chains, c = id - seg * chains, b = c / tiles;
+  uint32_t seg = 0;
+  const uint32_t c = blockIdx.x % chains, b = c / tiles;
+  if (tickets != nullptr) {
+    if (threadIdx.x == 0) *shared = atomicAdd(tickets + int64_t(c) * kTicketPitch, 1u);
+    __syncthreads();
+    seg = __builtin_amdgcn_readfirstlane(*shared);
+  }
   ScanPlace s;
   s.seg = seg;
   s.b = b;
@@ -229,10 +234,10 @@ __device__ __forceinline__ void exchange(const ScanArgs& p, const ScanPlace& s, 
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void k_scan_fwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
                                                   T* __restrict__ y, int64_t nseg, uint64_t* __restrict__ words,
-                                                  uint32_t* __restrict__ ticket) {
+                                                  uint32_t* __restrict__ tickets) {
   constexpr int K = chunk_steps<T>();
   __shared__ uint32_t shared;
-  const ScanPlace s = scan_place<VEC>(p, ticket, &shared);
+  const ScanPlace s = scan_place<VEC>(p, tickets, &shared);
   const bool live = s.d < p.D;
   const int64_t n = length_of(p.lengths, s.b, p.L), nck = (p.L + K - 1) / K, ck = s.seg * s.waves + s.wave, t0 = ck * K;
   const int rows = int(max(int64_t(0), min(int64_t(K), p.L - t0))), cnt = int(max(int64_t(0), min(int64_t(K), n - t0)));
@@ -283,10 +288,10 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(256) void k_scan_bwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
                                                   const T* __restrict__ dy, T* __restrict__ dx, T* __restrict__ dg,
                                                   int64_t nseg, uint64_t* __restrict__ words,
-                                                  uint32_t* __restrict__ ticket) {
+                                                  uint32_t* __restrict__ tickets) {
   constexpr int K = chunk_steps<T>();
   __shared__ uint32_t shared;
-  const ScanPlace s = scan_place<VEC>(p, ticket, &shared);
+  const ScanPlace s = scan_place<VEC>(p, tickets, &shared);
   const bool live = s.d < p.D;
   const int64_t seg = nseg - 1 - s.seg;  // time runs backwards along the tickets
   const int64_t n = length_of(p.lengths, s.b, p.L), nck = (p.L + K - 1) / K, ck = seg * s.waves + s.wave, t0 = ck * K;
@@ -373,7 +378,7 @@ __global__ __launch_bounds__(256) void k_scan_step(const T* __restrict__ x, int6
 
 struct ScanPlan {
   int waves = 1;
-  int64_t nseg = 1, blocks = 0;
+  int64_t nseg = 1, chains = 0, blocks = 0;
 };
 
 int chunk_of(int type) { return type == kF32 ? chunk_steps<float>() : chunk_steps<f16_t>(); }
@@ -385,7 +390,8 @@ ScanPlan scan_plan(const ScanArgs& p, int type, int vec, const char* who) {
   s.nseg = (chunks + s.waves - 1) / s.waves;
   const int64_t tiles = (p.D + kWave * vec - 1) / (kWave * vec);
   if (p.B > (int64_t(1) << 31) / tiles / s.nseg) throw std::invalid_argument(std::string(who) + ": too many elements");
-  s.blocks = p.B * tiles * s.nseg;
+  s.chains = p.B * tiles;
+  s.blocks = s.chains * s.nseg;
   return s;
 }
 
@@ -400,17 +406,17 @@ bool pairs(const ScanArgs& p, std::initializer_list<const void*> ptrs) {
   return true;
 }
 
-// Words not yet written, ticket 0: before a pass whose workgroups hand the state on.
+// Words not yet written, tickets 0: before a pass whose workgroups hand the state on.
 uint32_t* scan_begin(const ScanArgs& p, const ScanPlan& s, const char* who, hipStream_t stream) {
   if (s.nseg == 1) return nullptr;
   if (p.workspace == nullptr) throw std::invalid_argument(std::string(who) + ": no workspace");
   const int64_t n = scan_words(p, s);
   uint64_t* words = static_cast<uint64_t*>(p.workspace);
-  uint32_t* ticket = reinterpret_cast<uint32_t*>(words + n);
+  uint32_t* tickets = reinterpret_cast<uint32_t*>(words + n);
   hipLaunchKernelGGL(k_scan_init, dim3(uint32_t(std::min<int64_t>((n + 1023) / 1024, 2048))), dim3(256), 0, stream, words,
-                     n, ticket);
+                     n, tickets, s.chains);
   RMM_HIP_CHECK(hipGetLastError());
-  return ticket;
+  return tickets;
 }
 
 }  // namespace
@@ -421,8 +427,9 @@ int64_t gated_scan_workspace(int64_t B, int64_t L, int64_t D, int type) {
   ScanArgs p;
   p.B = B, p.L = L, p.D = D;
   if (B <= 0 || D <= 0) return 0;
-  const int64_t n = scan_words(p, scan_plan(p, type, 1, "gated_scan"));
-  return n ? n * int64_t(sizeof(uint64_t)) + 64 : 0;
+  const ScanPlan s = scan_plan(p, type, 1, "gated_scan");  // no more words and tickets than with pairs of channels
+  const int64_t n = scan_words(p, s);
+  return n ? n * int64_t(sizeof(uint64_t)) + s.chains * kTicketPitch * int64_t(sizeof(uint32_t)) : 0;
 }
 
 void gated_scan_fwd(const ScanArgs& p, const void* x, const void* g, void* y, int type, hipStream_t stream) {
@@ -431,15 +438,15 @@ void gated_scan_fwd(const ScanArgs& p, const void* x, const void* g, void* y, in
     using T = decltype(tag);
     const bool two = pairs<T>(p, {x, g, y});
     const ScanPlan s = scan_plan(p, type, two ? 2 : 1, "gated_scan");
-    uint32_t* ticket = scan_begin(p, s, "gated_scan", stream);
+    uint32_t* tickets = scan_begin(p, s, "gated_scan", stream);
     const dim3 grid(uint32_t(s.blocks)), block(uint32_t(s.waves * kWave));
     const T *xp = static_cast<const T*>(x), *gp = static_cast<const T*>(g);
     T* yp = static_cast<T*>(y);
     uint64_t* words = static_cast<uint64_t*>(p.workspace);
     if (two)
-      hipLaunchKernelGGL((k_scan_fwd<T, 2>), grid, block, 0, stream, p, xp, gp, yp, s.nseg, words, ticket);
+      hipLaunchKernelGGL((k_scan_fwd<T, 2>), grid, block, 0, stream, p, xp, gp, yp, s.nseg, words, tickets);
     else
-      hipLaunchKernelGGL((k_scan_fwd<T, 1>), grid, block, 0, stream, p, xp, gp, yp, s.nseg, words, ticket);
+      hipLaunchKernelGGL((k_scan_fwd<T, 1>), grid, block, 0, stream, p, xp, gp, yp, s.nseg, words, tickets);
   });
   RMM_HIP_CHECK(hipGetLastError());
 }
@@ -452,15 +459,15 @@ void gated_scan_bwd(const ScanArgs& p, const void* x, const void* g, const void*
     using T = decltype(tag);
     const bool two = pairs<T>(p, {x, g, dy, dx, dg});
     const ScanPlan s = scan_plan(p, type, two ? 2 : 1, "gated_scan backward");
-    uint32_t* ticket = scan_begin(p, s, "gated_scan backward", stream);
+    uint32_t* tickets = scan_begin(p, s, "gated_scan backward", stream);
     const dim3 grid(uint32_t(s.blocks)), block(uint32_t(s.waves * kWave));
     const T *xp = static_cast<const T*>(x), *gp = static_cast<const T*>(g), *yp = static_cast<const T*>(dy);
     T *dxp = static_cast<T*>(dx), *dgp = static_cast<T*>(dg);
     uint64_t* words = static_cast<uint64_t*>(p.workspace);
     if (two)
-      hipLaunchKernelGGL((k_scan_bwd<T, 2>), grid, block, 0, stream, p, xp, gp, yp, dxp, dgp, s.nseg, words, ticket);
+      hipLaunchKernelGGL((k_scan_bwd<T, 2>), grid, block, 0, stream, p, xp, gp, yp, dxp, dgp, s.nseg, words, tickets);
     else
-      hipLaunchKernelGGL((k_scan_bwd<T, 1>), grid, block, 0, stream, p, xp, gp, yp, dxp, dgp, s.nseg, words, ticket);
+      hipLaunchKernelGGL((k_scan_bwd<T, 1>), grid, block, 0, stream, p, xp, gp, yp, dxp, dgp, s.nseg, words, tickets);
   });
   RMM_HIP_CHECK(hipGetLastError());
 }

@@ -14,15 +14,11 @@
 //
 // Split. Either pass is a composition of affine maps s -> A s + H, one per step. A wave takes a chunk of K steps of
 // 64 VEC channels, loads it whole into registers (every load in flight at once) and composes its K maps per lane; the
-// 1 to 4 waves of a workgroup, consecutive chunks, exchange their compositions through LDS; and where a sequence is
-// longer than that, workgroups pass the state on in one launch: each publishes its composition as soon as it has it,
-// looks back over its predecessors' until it meets a finished state (each wave at other segments), publishes its own
-// finished state, and writes its rows. So x, g (and dy) cross the memory bus once for any L, and few channels still fill the card.
-//
-// Waiting. A published word is one 64-bit atomic (A, H) that carries its own readiness in A: all ones before it is
-// written, -1 for a finished state, else in [0, 1]. The workgroups of a chain (one sequence's 64 VEC channels) take their
-// segments from the chain's ticket counter, and wait only for lower tickets of that counter, whose workgroups therefore
-// run already: by induction over the tickets every wait ends.
+// up to 8 waves of a workgroup take consecutive chunks, exchange their compositions through LDS, and go on to the next
+// tile of chunks with the state behind this one, whose loads they issued before the exchange. With enough chains (one
+// sequence's 64 VEC channels) to fill the card, that reads x, g (and dy) once. With fewer, a chain is cut into segments:
+// k_scan_maps composes the map of each from a first reading, and the workgroups of the pass itself start from the maps
+// before theirs.
 //
 // A = 0 stands for a reset alone: what is before it is dropped, not multiplied by zero (it may be infinite or NaN).
 // Products that underflow are held at the smallest denormal instead, so an infinite state stays infinite.
@@ -40,7 +36,7 @@ namespace hip {
 
 namespace {
 
-constexpr int kScanWaves = 4;  // most waves of a workgroup
+constexpr int kScanWaves = 8, kScanThreads = kScanWaves * kWave;  // most waves of a workgroup
 constexpr float kTiny = 1.4e-45f;
 
 template <typename T>
@@ -74,87 +70,23 @@ __device__ __forceinline__ Map then(const Map& first, const Map& later) {
   return Map{first.A == 0.f ? 0.f : fmaxf(first.A * later.A, kTiny), fmaf(later.A, first.H, later.H)};
 }
 
-__device__ __forceinline__ uint64_t pack(float a, float h) {
-  return (uint64_t(__float_as_uint(a)) << 32) | __float_as_uint(h);
-}
-
-__device__ __forceinline__ uint64_t peek(const uint64_t* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-__device__ __forceinline__ void publish(uint64_t* p, uint64_t v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-constexpr int kTicketPitch = 32;  // counters a cache line apart
-
-__global__ __launch_bounds__(256) void k_scan_init(uint64_t* __restrict__ words, int64_t n,
-                                                   uint32_t* __restrict__ tickets, int64_t chains) {
-  const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x, step = int64_t(gridDim.x) * 256;
-  for (int64_t i = at; i < n; i += step) words[i] = ~0ull;
-  for (int64_t i = at; i < chains; i += step) tickets[i * kTicketPitch] = 0;
-}
-
-// What the words of up to `depth` segments j, j - 1, .. of VEC neighbouring chains say about the state behind segment j:
-// the composition of their maps, or, once a finished state is met, that state carried through them (A = kDone). The words
-// do not depend on each other, so all are read at once. Segments below 0 do not exist: segment 0 always finishes.
-constexpr int kLook = 8;
-constexpr float kDone = -1.f;
-template <int VEC>
-__device__ __forceinline__ void look_back(const uint64_t* __restrict__ word, int j, int depth, int64_t stride,
-                                          Map (&acc)[VEC]) {
-  uint64_t w[kLook][VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; v++) acc[v] = Map{1.f, 0.f};
-#pragma unroll
-  for (int q = 0; q < kLook; q++) {
-    if (q < depth && j - q >= 0) {
-#pragma unroll
-      for (int v = 0; v < VEC; v++) w[q][v] = peek(word + (j - q) * stride + v);
-    }
-  }
-#pragma unroll
-  for (int q = 0; q < kLook; q++) {
-    if (q < depth && j - q >= 0) {
-#pragma unroll
-      for (int v = 0; v < VEC; v++) {
-        if (acc[v].A == kDone) continue;
-        while (uint32_t(w[q][v] >> 32) == 0xFFFFFFFFu) {
-          __builtin_amdgcn_s_sleep(1);
-          w[q][v] = peek(word + (j - q) * stride + v);
-        }
-        const Map m{__uint_as_float(uint32_t(w[q][v] >> 32)), __uint_as_float(uint32_t(w[q][v]))};
-        acc[v] = m.A == kDone ? Map{kDone, apply(acc[v], m.H)} : then(m, acc[v]);
-        if (acc[v].A == 0.f) acc[v].A = kDone;  // nothing before a reset matters
-      }
-    }
-  }
-}
-
+// Which sequence, channels and segment a workgroup has, and where its wave stands.
 struct ScanPlace {
   int64_t b, d;
   int seg, wave, lane, waves;
 };
 
-// Which (sequence, channels, segment) this workgroup has. Neighbouring workgroups are of different chains, so a chain's
-// segments start as far apart as the number of chains allows.
 template <int VEC>
-__device__ __forceinline__ ScanPlace scan_place(const ScanArgs& p, uint32_t* __restrict__ tickets, uint32_t* shared) {
+__device__ __forceinline__ ScanPlace scan_place(const ScanArgs& p) {
   const uint32_t tiles = uint32_t((p.D + kWave * VEC - 1) / (kWave * VEC)), chains = uint32_t(p.B) * tiles;
-  uint32_t seg = 0;
-  const uint32_t c = blockIdx.x % chains, b = c / tiles;
-  if (tickets != nullptr) {
-    if (threadIdx.x == 0) *shared = atomicAdd(tickets + int64_t(c) * kTicketPitch, 1u);
-    __syncthreads();
-    seg = __builtin_amdgcn_readfirstlane(*shared);
-  }
+  const uint32_t seg = blockIdx.x / chains, chain = blockIdx.x - seg * chains, b = chain / tiles;
   ScanPlace s;
   s.seg = int(seg);
   s.b = b;
   s.lane = threadIdx.x % kWave;
   s.wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   s.waves = blockDim.x / kWave;
-  s.d = (int64_t(c - b * tiles) * kWave + s.lane) * VEC;
+  s.d = (int64_t(chain - b * tiles) * kWave + s.lane) * VEC;
   return s;
 }
 
@@ -176,72 +108,41 @@ __device__ __forceinline__ void load_rows(const T* __restrict__ p, int64_t strid
   }
 }
 
-// The state that enters each wave's chunk (`in`), from the waves' compositions and what enters the workgroup, and the
-// state behind the workgroup (`last`). The waves look back at different segments at the same time, `depth` each.
+// The state that enters this wave's chunk, from the state before the tile (`carry`, which goes on to that behind it) and
+// the compositions of the tile's waves, in the order of the recurrence. `maps` alternates between two buffers from tile to
+// tile, so that one barrier a tile is enough.
 template <int VEC>
-__device__ __forceinline__ void exchange(const ScanArgs& p, const ScanPlace& s, bool forward, int seg, int nseg, int depth,
-                                         const float* __restrict__ start, uint64_t* __restrict__ words,
-                                         const Map (&mine)[VEC], float (&in)[VEC], float (&last)[VEC]) {
-  __shared__ Map maps[kScanWaves][kWave * VEC];
-  __shared__ Map seen[2][kScanWaves][kWave * VEC];
-  const bool live = s.d < p.D;
+__device__ __forceinline__ void exchange(const ScanPlace& s, bool forward, Map (*maps)[kWave * VEC], const Map (&mine)[VEC],
+                                         float (&carry)[VEC], float (&in)[VEC]) {
   const int at = s.lane * VEC;
 #pragma unroll
   for (int v = 0; v < VEC; v++) maps[s.wave][at + v] = mine[v];
   __syncthreads();
-  const int64_t dp = (p.D + 127) / 128 * 128, stride = p.B * dp;
-  uint64_t* word = words + s.b * dp + s.d;
-  Map all[VEC];
+  for (int k = 0; k < s.waves; k++) {
+    const int w = forward ? k : s.waves - 1 - k;
 #pragma unroll
-  for (int v = 0; v < VEC; v++) {
-    all[v] = Map{1.f, 0.f};
-    for (int k = 0; k < s.waves; k++) all[v] = then(all[v], maps[forward ? k : s.waves - 1 - k][at + v]);
-  }
-  if (seg == 0) {
-#pragma unroll
-    for (int v = 0; v < VEC; v++) in[v] = live && start ? start[s.b * p.D + s.d + v] : 0.f;
-  } else {
-    if (s.wave == 0 && live) {
-#pragma unroll
-      for (int v = 0; v < VEC; v++) publish(word + seg * stride + v, pack(all[v].A, all[v].H));
+    for (int v = 0; v < VEC; v++) {
+      if (w == s.wave) in[v] = carry[v];
+      carry[v] = apply(maps[w][at + v], carry[v]);
     }
-    Map acc[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; v++) acc[v] = Map{live ? 1.f : kDone, 0.f};
-    // every wave follows the same joined composition, so all leave after the same round
-    bool more = true;
-    for (int j = seg - 1, round = 0; more; j -= s.waves * depth, round ^= 1) {
-      Map found[VEC];
-      if (live) look_back<VEC>(word, j - s.wave * depth, depth, stride, found);
-#pragma unroll
-      for (int v = 0; v < VEC; v++) seen[round][s.wave][at + v] = found[v];
-      __syncthreads();
-      bool open = false;
-#pragma unroll
-      for (int v = 0; v < VEC; v++) {
-        for (int k = 0; k < s.waves; k++) {
-          const Map m = seen[round][k][at + v];
-          if (acc[v].A != kDone) {
-            acc[v] = m.A == kDone ? Map{kDone, apply(acc[v], m.H)} : then(m, acc[v]);
-          }
-        }
-        open = open || acc[v].A != kDone;
-      }
-      more = __any(open);
-    }
-#pragma unroll
-    for (int v = 0; v < VEC; v++) in[v] = acc[v].H;
   }
+}
+
+// The state before segment `seg` in the order of the recurrence: the chain's start carried through the maps of the
+// segments before it.
+template <int VEC>
+__device__ __forceinline__ void start_state(const ScanArgs& p, const ScanPlace& s, int seg, const float* __restrict__ start,
+                                            const Map* __restrict__ maps, float (&state)[VEC]) {
+  const bool live = s.d < p.D;
 #pragma unroll
-  for (int v = 0; v < VEC; v++) last[v] = apply(all[v], in[v]);
-  if (nseg > 1 && s.wave == 0 && live) {
+  for (int v = 0; v < VEC; v++) state[v] = live && start ? start[s.b * p.D + s.d + v] : 0.f;
+  if (!live) return;
+  const Map* m = maps + s.b * p.D + s.d;
+#pragma unroll 8
+  for (int k = 0; k < seg; k++) {
 #pragma unroll
-    for (int v = 0; v < VEC; v++) publish(word + seg * stride + v, pack(kDone, last[v]));
+    for (int v = 0; v < VEC; v++) state[v] = apply(m[k * p.B * p.D + v], state[v]);
   }
-  const int before = forward ? s.wave : s.waves - 1 - s.wave;  // chunks of this workgroup that come before mine
-#pragma unroll
-  for (int v = 0; v < VEC; v++)
-    for (int k = 0; k < before; k++) in[v] = apply(maps[forward ? k : s.waves - 1 - k][at + v], in[v]);
 }
 
 // The steps of a chunk: how many lie inside the tensor, how many of them belong to the sequence, which have a reset.
@@ -252,10 +153,10 @@ struct Chunk {
 };
 
 template <int K>
-__device__ __forceinline__ Chunk chunk_of(const ScanArgs& p, const ScanPlace& s, int seg) {
+__device__ __forceinline__ Chunk chunk_of(const ScanArgs& p, const ScanPlace& s, int n, int ck) {
   Chunk c;
-  c.ck = seg * s.waves + s.wave;
-  const int L = int(p.L), t0 = c.ck * K, n = length_of(p.lengths, s.b, L);
+  c.ck = ck;
+  const int L = int(p.L), t0 = ck * K;
   c.t0 = t0;
   c.rows = max(0, min(K, L - t0));
   c.cnt = max(0, min(K, n - t0));
@@ -305,39 +206,54 @@ __device__ __forceinline__ void write_states(const Chunk& c, const float (&ca)[K
   }
 }
 
+// `per` tiles in a segment.
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void k_scan_fwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
-                                                  T* __restrict__ y, int nseg, int depth, uint64_t* __restrict__ words,
-                                                  uint32_t* __restrict__ tickets) {
+__global__ __launch_bounds__(kScanThreads) void k_scan_fwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
+                                                           T* __restrict__ y, int nseg, int per,
+                                                           const Map* __restrict__ seg_maps) {
   constexpr int K = chunk_steps<T>();
-  __shared__ uint32_t shared;
-  const ScanPlace s = scan_place<VEC>(p, tickets, &shared);
+  __shared__ Map maps[2][kScanWaves][kWave * VEC];
+  const ScanPlace s = scan_place<VEC>(p);
   const bool live = s.d < p.D;
-  const Chunk c = chunk_of<K>(p, s, s.seg);
+  const int n = length_of(p.lengths, s.b, int(p.L)), nck = int((p.L + K - 1) / K);
+  const int first = s.seg * per, last = max(first + 1, min(first + per, (nck + s.waves - 1) / s.waves));
+  const T *xp = x + s.b * p.xsb + s.d, *gp = g + s.b * p.gsb + s.d;
   VecOf<T, VEC> xr[K], gr[K];
+  Chunk c = chunk_of<K>(p, s, n, first * s.waves + s.wave);
   if (live) {
-    load_rows<T, VEC, K>(x + s.b * p.xsb + c.t0 * p.xst + s.d, p.xst, c.cnt, xr);
-    load_rows<T, VEC, K>(g + s.b * p.gsb + c.t0 * p.gst + s.d, p.gst, c.cnt, gr);
+    load_rows<T, VEC, K>(gp + c.t0 * p.gst, p.gst, c.cnt, gr);
+    load_rows<T, VEC, K>(xp + c.t0 * p.xst, p.xst, c.cnt, xr);
   }
-  float ca[K][VEC], ch[K][VEC];
-  Map m[VEC];
+  float carry[VEC];
+  start_state<VEC>(p, s, s.seg, p.h0, seg_maps, carry);
+  for (int tile = first; tile < last; tile++) {
+    float ca[K][VEC], ch[K][VEC], in[VEC];
+    Map m[VEC];
 #pragma unroll
-  for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
-  const bool plain = c.cnt == K && c.resets == 0;
-  if (plain)
-    compose<true, T, VEC, K>(c, xr, gr, ca, ch, m);
-  else
-    compose<false, T, VEC, K>(c, xr, gr, ca, ch, m);
-  float in[VEC], last[VEC];
-  exchange<VEC>(p, s, true, s.seg, nseg, depth, p.h0, words, m, in, last);
-  if (!live) return;
-  if (s.wave == 0 && s.seg == nseg - 1) store_vec<float, VEC>(p.h_last + s.b * p.D + s.d, last);
-  if (c.rows > 0 && p.ckpt) store_vec<float, VEC>(p.ckpt + (s.b * ((p.L + K - 1) / K) + c.ck) * p.D + s.d, in);
-  T* yp = y + (s.b * p.L + c.t0) * p.D + s.d;
-  if (plain)
-    write_states<true, T, VEC, K>(c, ca, ch, in, yp, p.D);
-  else
-    write_states<false, T, VEC, K>(c, ca, ch, in, yp, p.D);
+    for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
+    const Chunk now = c;
+    const bool plain = now.cnt == K && now.resets == 0;
+    if (plain)
+      compose<true, T, VEC, K>(now, xr, gr, ca, ch, m);
+    else
+      compose<false, T, VEC, K>(now, xr, gr, ca, ch, m);
+    if (tile + 1 < last) {
+      c = chunk_of<K>(p, s, n, (tile + 1) * s.waves + s.wave);
+      if (live) {
+        load_rows<T, VEC, K>(gp + c.t0 * p.gst, p.gst, c.cnt, gr);
+        load_rows<T, VEC, K>(xp + c.t0 * p.xst, p.xst, c.cnt, xr);
+      }
+    }
+    exchange<VEC>(s, true, maps[tile & 1], m, carry, in);
+    if (!live) continue;
+    if (now.rows > 0 && p.ckpt) store_vec<float, VEC>(p.ckpt + (s.b * nck + now.ck) * p.D + s.d, in);
+    T* yp = y + (s.b * p.L + now.t0) * p.D + s.d;
+    if (plain)
+      write_states<true, T, VEC, K>(now, ca, ch, in, yp, p.D);
+    else
+      write_states<false, T, VEC, K>(now, ca, ch, in, yp, p.D);
+  }
+  if (live && s.wave == 0 && s.seg == nseg - 1) store_vec<float, VEC>(p.h_last + s.b * p.D + s.d, carry);
 }
 
 // One chunk backward: z, the gate's factor dg / dh (cc) and, running against time, the composition of what reaches the
@@ -398,43 +314,106 @@ __device__ __forceinline__ void write_grads(const Chunk& c, const float (&zz)[K]
 }
 
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void k_scan_bwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
-                                                  const T* __restrict__ dy, T* __restrict__ dx, T* __restrict__ dg,
-                                                  int nseg, int depth, uint64_t* __restrict__ words,
-                                                  uint32_t* __restrict__ tickets) {
+__global__ __launch_bounds__(kScanThreads) void k_scan_bwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
+                                                           const T* __restrict__ dy, T* __restrict__ dx,
+                                                           T* __restrict__ dg, int nseg, int per,
+                                                           const Map* __restrict__ seg_maps) {
   constexpr int K = chunk_steps<T>();
-  __shared__ uint32_t shared;
-  const ScanPlace s = scan_place<VEC>(p, tickets, &shared);
+  __shared__ Map maps[2][kScanWaves][kWave * VEC];
+  const ScanPlace s = scan_place<VEC>(p);  // segment 0 is the last in time, where this pass begins
   const bool live = s.d < p.D;
-  const Chunk c = chunk_of<K>(p, s, nseg - 1 - s.seg);  // time runs backwards along the tickets
+  const int n = length_of(p.lengths, s.b, int(p.L)), nck = int((p.L + K - 1) / K);
+  const int first = (nseg - 1 - s.seg) * per, last = max(first + 1, min(first + per, (nck + s.waves - 1) / s.waves));
+  const T *xp = x + s.b * p.xsb + s.d, *gp = g + s.b * p.gsb + s.d, *yp = dy + s.b * p.ysb + s.d;
   VecOf<T, VEC> xr[K], gr[K], yr[K];
-  float h[VEC];
+  float h[VEC] = {};
+  Chunk c;
+  const auto load = [&](int tile) {
+    c = chunk_of<K>(p, s, n, tile * s.waves + s.wave);
+    if (!live) return;
+    if (c.cnt > 0) load_vec<float, VEC>(p.ckpt + (s.b * nck + c.ck) * p.D + s.d, h);
+    load_rows<T, VEC, K>(gp + c.t0 * p.gst, p.gst, c.cnt, gr);
+    load_rows<T, VEC, K>(xp + c.t0 * p.xst, p.xst, c.cnt, xr);
+    if (dy) load_rows<T, VEC, K>(yp + c.t0 * p.yst, p.yst, c.cnt, yr);
+  };
+  load(last - 1);
+  float carry[VEC];
+  start_state<VEC>(p, s, s.seg, p.dh_last, seg_maps, carry);
+  for (int tile = last - 1; tile >= first; tile--) {
+    float zz[K][VEC], cc[K][VEC], aa[K][VEC], dh[K][VEC], in[VEC];
+    Map m[VEC];
 #pragma unroll
-  for (int v = 0; v < VEC; v++) h[v] = 0.f;
-  if (live) {
-    if (c.rows > 0) load_vec<float, VEC>(p.ckpt + (s.b * ((p.L + K - 1) / K) + c.ck) * p.D + s.d, h);
-    load_rows<T, VEC, K>(g + s.b * p.gsb + c.t0 * p.gst + s.d, p.gst, c.cnt, gr);
-    load_rows<T, VEC, K>(x + s.b * p.xsb + c.t0 * p.xst + s.d, p.xst, c.cnt, xr);
-    if (dy) load_rows<T, VEC, K>(dy + s.b * p.ysb + c.t0 * p.yst + s.d, p.yst, c.cnt, yr);
+    for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
+    const Chunk now = c;
+    const bool plain = now.cnt == K && now.resets == 0 && dy != nullptr;
+    if (plain)
+      compose_back<true, T, VEC, K>(now, xr, gr, yr, true, h, zz, cc, aa, dh, m);
+    else
+      compose_back<false, T, VEC, K>(now, xr, gr, yr, dy != nullptr, h, zz, cc, aa, dh, m);
+    if (tile > first) load(tile - 1);
+    exchange<VEC>(s, false, maps[tile & 1], m, carry, in);
+    if (!live) continue;
+    T *dxp = dx + s.b * p.dsb + now.t0 * p.dst + s.d, *dgp = dg + s.b * p.dsb + now.t0 * p.dst + s.d;
+    if (plain)
+      write_grads<true, T, VEC, K>(now, zz, cc, aa, dh, in, dxp, dgp, p.dst);
+    else
+      write_grads<false, T, VEC, K>(now, zz, cc, aa, dh, in, dxp, dgp, p.dst);
   }
-  float zz[K][VEC], cc[K][VEC], aa[K][VEC], dh[K][VEC];
+  if (live && p.dh0 && s.wave == 0 && s.seg == nseg - 1) store_vec<float, VEC>(p.dh0 + s.b * p.D + s.d, carry);
+}
+
+// The maps of all segments but the last, in the order of the recurrence: forward of (gate, input), backward of
+// (gate, dy). Each wave composes a run of neighbouring chunks on its own; the runs are joined at the end.
+template <typename T, int VEC, bool FORWARD>
+__global__ __launch_bounds__(kScanThreads) void k_scan_maps(ScanArgs p, const T* __restrict__ g, const T* __restrict__ in,
+                                                            int nseg, int per, Map* __restrict__ seg_maps) {
+  constexpr int K = chunk_steps<T>();
+  __shared__ Map maps[kScanWaves][kWave * VEC];
+  const ScanPlace s = scan_place<VEC>(p);
+  const bool live = s.d < p.D;
+  const int n = length_of(p.lengths, s.b, int(p.L)), nck = int((p.L + K - 1) / K);
+  const int seg = FORWARD ? s.seg : nseg - 1 - s.seg;  // in time; a tile has s.waves chunks, so a wave's run has `per`
+  const int lo = seg * per * s.waves + s.wave * per, hi = min(lo + per, nck);
+  const int64_t isb = FORWARD ? p.xsb : p.ysb, ist = FORWARD ? p.xst : p.yst;
+  const T *gp = g + s.b * p.gsb + s.d, *ip = in + s.b * isb + s.d;
   Map m[VEC];
 #pragma unroll
   for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
-  const bool plain = c.cnt == K && c.resets == 0 && dy != nullptr;
-  if (plain)
-    compose_back<true, T, VEC, K>(c, xr, gr, yr, true, h, zz, cc, aa, dh, m);
-  else
-    compose_back<false, T, VEC, K>(c, xr, gr, yr, dy != nullptr, h, zz, cc, aa, dh, m);
-  float in[VEC], last[VEC];
-  exchange<VEC>(p, s, false, s.seg, nseg, depth, p.dh_last, words, m, in, last);
-  if (!live) return;
-  if (p.dh0 && s.wave == 0 && s.seg == nseg - 1) store_vec<float, VEC>(p.dh0 + s.b * p.D + s.d, last);
-  T *xp = dx + s.b * p.dsb + c.t0 * p.dst + s.d, *gp = dg + s.b * p.dsb + c.t0 * p.dst + s.d;
-  if (plain)
-    write_grads<true, T, VEC, K>(c, zz, cc, aa, dh, in, xp, gp, p.dst);
-  else
-    write_grads<false, T, VEC, K>(c, zz, cc, aa, dh, in, xp, gp, p.dst);
+  for (int k = 0; k < hi - lo; k++) {
+    const Chunk c = chunk_of<K>(p, s, n, FORWARD ? lo + k : hi - 1 - k);
+    if (!live || c.cnt == 0) continue;
+    VecOf<T, VEC> gr[K], ir[K];
+    load_rows<T, VEC, K>(gp + c.t0 * p.gst, p.gst, c.cnt, gr);
+    if (in) load_rows<T, VEC, K>(ip + c.t0 * ist, ist, c.cnt, ir);
+#pragma unroll
+    for (int q = 0; q < K; q++) {
+      const int i = FORWARD ? q : K - 1 - q;
+      const bool drop = (c.resets >> i) & 1;
+#pragma unroll
+      for (int v = 0; v < VEC; v++) {
+        if (i < c.cnt) {
+          float z, a;
+          gate_of(to_f32(gr[i].v[v]), z, a);
+          const float iv = in ? to_f32(ir[i].v[v]) : 0.f;
+          if (FORWARD)
+            m[v].H = drop ? z * iv : fmaf(a, m[v].H, z * iv);
+          else
+            m[v].H = drop ? 0.f : a * (m[v].H + iv);
+          m[v].A = drop || m[v].A == 0.f ? 0.f : fmaxf(m[v].A * a, kTiny);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < VEC; v++) maps[s.wave][s.lane * VEC + v] = m[v];
+  __syncthreads();
+  if (s.wave != 0 || !live) return;
+#pragma unroll
+  for (int v = 0; v < VEC; v++) {
+    Map all{1.f, 0.f};
+    for (int k = 0; k < s.waves; k++) all = then(all, maps[FORWARD ? k : s.waves - 1 - k][s.lane * VEC + v]);
+    seg_maps[(s.seg * p.B + s.b) * p.D + s.d + v] = all;
+  }
 }
 
 template <typename T>
@@ -453,28 +432,28 @@ __global__ __launch_bounds__(256) void k_scan_step(const T* __restrict__ x, int6
 }
 
 struct ScanPlan {
-  int waves = 1, depth = 1;
-  int64_t nseg = 1, chains = 0, blocks = 0;
+  int waves = 1, per = 1, nseg = 1;
+  int64_t chains = 0;
 };
 
 int steps_of(int type) { return type == kF32 ? chunk_steps<float>() : chunk_steps<f16_t>(); }
 
+// Workgroups that the passes want before they cut no chain, and that they cut towards.
+constexpr int64_t kEnoughChains = 160, kWantGroups = 512;
+
 ScanPlan scan_plan(const ScanArgs& p, int type, int vec, const char* who) {
+  if (p.L >= (int64_t(1) << 31) - 4096) throw std::invalid_argument(std::string(who) + ": too many steps");
   ScanPlan s;
-  if (p.L >= (int64_t(1) << 31) - 64) throw std::invalid_argument(std::string(who) + ": too many steps");
   const int64_t chunks = std::max<int64_t>(1, (p.L + steps_of(type) - 1) / steps_of(type));
   s.waves = int(std::min<int64_t>(kScanWaves, chunks));
-  s.nseg = (chunks + s.waves - 1) / s.waves;
-  const int64_t tiles = (p.D + kWave * vec - 1) / (kWave * vec);
-  if (p.B > (int64_t(1) << 31) / tiles / s.nseg) throw std::invalid_argument(std::string(who) + ": too many elements");
-  s.chains = p.B * tiles;
-  s.blocks = s.chains * s.nseg;
-  // about 1024 workgroups run at a time, so that many / chains segments of a chain are unfinished
-  s.depth = int(std::max<int64_t>(1, std::min<int64_t>(kLook, 1024 / kScanWaves / s.chains)));
+  const int64_t tiles = (chunks + s.waves - 1) / s.waves, cols = (p.D + kWave * vec - 1) / (kWave * vec);
+  if (p.B > (int64_t(1) << 31) / cols / 1024) throw std::invalid_argument(std::string(who) + ": too many sequences");
+  s.chains = p.B * cols;
+  int64_t nseg = s.chains >= kEnoughChains ? 1 : std::min(tiles, (kWantGroups + s.chains - 1) / s.chains);
+  s.per = int((tiles + nseg - 1) / nseg);
+  s.nseg = int((tiles + s.per - 1) / s.per);
   return s;
 }
-
-int64_t scan_words(const ScanArgs& p, const ScanPlan& s) { return s.nseg == 1 ? 0 : s.nseg * p.B * ((p.D + 127) / 128 * 128); }
 
 // Two channels a lane where every row of every tensor starts at a multiple of two elements.
 template <typename T>
@@ -485,17 +464,34 @@ bool pairs(const ScanArgs& p, std::initializer_list<const void*> ptrs) {
   return true;
 }
 
-// Words not yet written, tickets 0: before a pass whose workgroups hand the state on.
-uint32_t* scan_begin(const ScanArgs& p, const ScanPlan& s, const char* who, hipStream_t stream) {
-  if (s.nseg == 1) return nullptr;
-  if (p.workspace == nullptr) throw std::invalid_argument(std::string(who) + ": no workspace");
-  const int64_t n = scan_words(p, s);
-  uint64_t* words = static_cast<uint64_t*>(p.workspace);
-  uint32_t* tickets = reinterpret_cast<uint32_t*>(words + n);
-  hipLaunchKernelGGL(k_scan_init, dim3(uint32_t(std::min<int64_t>((n + 1023) / 1024, 2048))), dim3(256), 0, stream, words,
-                     n, tickets, s.chains);
+template <typename T, int VEC>
+void scan_fwd_t(const ScanArgs& p, const T* x, const T* g, T* y, int type, hipStream_t stream) {
+  const ScanPlan s = scan_plan(p, type, VEC, "gated_scan");
+  Map* maps = static_cast<Map*>(p.workspace);
+  const dim3 block(uint32_t(s.waves * kWave));
+  if (s.nseg > 1) {
+    if (maps == nullptr) throw std::invalid_argument("gated_scan: no workspace");
+    hipLaunchKernelGGL((k_scan_maps<T, VEC, true>), dim3(uint32_t(s.chains * (s.nseg - 1))), block, 0, stream, p, g, x,
+                       s.nseg, s.per, maps);
+  }
+  hipLaunchKernelGGL((k_scan_fwd<T, VEC>), dim3(uint32_t(s.chains * s.nseg)), block, 0, stream, p, x, g, y, s.nseg, s.per,
+                     maps);
   RMM_HIP_CHECK(hipGetLastError());
-  return tickets;
+}
+
+template <typename T, int VEC>
+void scan_bwd_t(const ScanArgs& p, const T* x, const T* g, const T* dy, T* dx, T* dg, int type, hipStream_t stream) {
+  const ScanPlan s = scan_plan(p, type, VEC, "gated_scan backward");
+  Map* maps = static_cast<Map*>(p.workspace);
+  const dim3 block(uint32_t(s.waves * kWave));
+  if (s.nseg > 1) {
+    if (maps == nullptr) throw std::invalid_argument("gated_scan backward: no workspace");
+    hipLaunchKernelGGL((k_scan_maps<T, VEC, false>), dim3(uint32_t(s.chains * (s.nseg - 1))), block, 0, stream, p, g, dy,
+                       s.nseg, s.per, maps);
+  }
+  hipLaunchKernelGGL((k_scan_bwd<T, VEC>), dim3(uint32_t(s.chains * s.nseg)), block, 0, stream, p, x, g, dy, dx, dg, s.nseg,
+                     s.per, maps);
+  RMM_HIP_CHECK(hipGetLastError());
 }
 
 }  // namespace
@@ -506,28 +502,17 @@ int64_t gated_scan_workspace(int64_t B, int64_t L, int64_t D, int type) {
   ScanArgs p;
   p.B = B, p.L = L, p.D = D;
   if (B <= 0 || D <= 0) return 0;
-  const ScanPlan s = scan_plan(p, type, 1, "gated_scan");  // no more words and tickets than with pairs of channels
-  const int64_t n = scan_words(p, s);
-  return n ? n * int64_t(sizeof(uint64_t)) + s.chains * kTicketPitch * int64_t(sizeof(uint32_t)) : 0;
+  const int nseg = std::max(scan_plan(p, type, 1, "gated_scan").nseg, scan_plan(p, type, 2, "gated_scan").nseg);
+  return nseg == 1 ? 0 : (nseg - 1) * B * D * int64_t(sizeof(Map));
 }
 
 void gated_scan_fwd(const ScanArgs& p, const void* x, const void* g, void* y, int type, hipStream_t stream) {
   if (p.B <= 0 || p.D <= 0) return;
   dispatch_type(type, "gated_scan", [&](auto tag) {
     using T = decltype(tag);
-    const bool two = pairs<T>(p, {x, g, y});
-    const ScanPlan s = scan_plan(p, type, two ? 2 : 1, "gated_scan");
-    uint32_t* tickets = scan_begin(p, s, "gated_scan", stream);
-    const dim3 grid(uint32_t(s.blocks)), block(uint32_t(s.waves * kWave));
-    const T *xp = static_cast<const T*>(x), *gp = static_cast<const T*>(g);
-    T* yp = static_cast<T*>(y);
-    uint64_t* words = static_cast<uint64_t*>(p.workspace);
-    if (two)
-      hipLaunchKernelGGL((k_scan_fwd<T, 2>), grid, block, 0, stream, p, xp, gp, yp, int(s.nseg), s.depth, words, tickets);
-    else
-      hipLaunchKernelGGL((k_scan_fwd<T, 1>), grid, block, 0, stream, p, xp, gp, yp, int(s.nseg), s.depth, words, tickets);
+    const auto fwd = pairs<T>(p, {x, g, y}) ? scan_fwd_t<T, 2> : scan_fwd_t<T, 1>;
+    fwd(p, static_cast<const T*>(x), static_cast<const T*>(g), static_cast<T*>(y), type, stream);
   });
-  RMM_HIP_CHECK(hipGetLastError());
 }
 
 void gated_scan_bwd(const ScanArgs& p, const void* x, const void* g, const void* dy, void* dx, void* dg, int type,
@@ -536,19 +521,10 @@ void gated_scan_bwd(const ScanArgs& p, const void* x, const void* g, const void*
   if (p.L > 0 && p.ckpt == nullptr) throw std::invalid_argument("gated_scan backward: no saved states");
   dispatch_type(type, "gated_scan backward", [&](auto tag) {
     using T = decltype(tag);
-    const bool two = pairs<T>(p, {x, g, dy, dx, dg});
-    const ScanPlan s = scan_plan(p, type, two ? 2 : 1, "gated_scan backward");
-    uint32_t* tickets = scan_begin(p, s, "gated_scan backward", stream);
-    const dim3 grid(uint32_t(s.blocks)), block(uint32_t(s.waves * kWave));
-    const T *xp = static_cast<const T*>(x), *gp = static_cast<const T*>(g), *yp = static_cast<const T*>(dy);
-    T *dxp = static_cast<T*>(dx), *dgp = static_cast<T*>(dg);
-    uint64_t* words = static_cast<uint64_t*>(p.workspace);
-    if (two)
-      hipLaunchKernelGGL((k_scan_bwd<T, 2>), grid, block, 0, stream, p, xp, gp, yp, dxp, dgp, int(s.nseg), s.depth, words, tickets);
-    else
-      hipLaunchKernelGGL((k_scan_bwd<T, 1>), grid, block, 0, stream, p, xp, gp, yp, dxp, dgp, int(s.nseg), s.depth, words, tickets);
+    const auto bwd = pairs<T>(p, {x, g, dy, dx, dg}) ? scan_bwd_t<T, 2> : scan_bwd_t<T, 1>;
+    bwd(p, static_cast<const T*>(x), static_cast<const T*>(g), static_cast<const T*>(dy), static_cast<T*>(dx),
+        static_cast<T*>(dg), type, stream);
   });
-  RMM_HIP_CHECK(hipGetLastError());
 }
 
 void gated_scan_step(const void* x, int64_t xs, const void* g, int64_t gs, const uint8_t* resets, const float* h,

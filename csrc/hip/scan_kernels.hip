@@ -164,43 +164,48 @@ __device__ __forceinline__ Chunk chunk_of(const ScanArgs& p, const ScanPlace& s,
   return c;
 }
 
-// One chunk forward: ca, ch become the composition up to each step, m that of the chunk. PLAIN: all K steps and no reset.
+// The chunk's factor of the state before it, from the plain product of its steps' factors.
+__device__ __forceinline__ float chunk_factor(const Chunk& c, float product) {
+  return c.resets ? 0.f : fmaxf(product, kTiny);
+}
+
+// One chunk forward: 1 - z and z x of each step, and the chunk's map. PLAIN: all K steps and no reset.
 template <bool PLAIN, typename T, int VEC, int K>
 __device__ __forceinline__ void compose(const Chunk& c, const VecOf<T, VEC> (&x)[K], const VecOf<T, VEC> (&g)[K],
-                                        float (&ca)[K][VEC], float (&ch)[K][VEC], Map (&m)[VEC]) {
+                                        float (&aa)[K][VEC], float (&uu)[K][VEC], Map (&m)[VEC]) {
+#pragma unroll
+  for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
 #pragma unroll
   for (int i = 0; i < K; i++) {
-    const bool drop = !PLAIN && ((c.resets >> i) & 1), dropped = !PLAIN && (c.resets & ((2u << i) - 1)) != 0;
+    const bool drop = !PLAIN && ((c.resets >> i) & 1);
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
       if (PLAIN || i < c.cnt) {
-        float z, a;
-        gate_of(to_f32(g[i].v[v]), z, a);
-        const float u = z * to_f32(x[i].v[v]);
-        m[v].H = drop ? u : fmaf(a, m[v].H, u);
-        m[v].A = dropped ? 0.f : fmaxf(m[v].A * a, kTiny);
+        float z;
+        gate_of(to_f32(g[i].v[v]), z, aa[i][v]);
+        uu[i][v] = z * to_f32(x[i].v[v]);
+        m[v].H = drop ? uu[i][v] : fmaf(aa[i][v], m[v].H, uu[i][v]);
+        m[v].A *= aa[i][v];
       }
-      ca[i][v] = m[v].A;
-      ch[i][v] = m[v].H;
     }
   }
-}
-
-// s carried through the composition (a, h), which has no reset in it where PLAIN.
-template <bool PLAIN>
-__device__ __forceinline__ float carry(float a, float h, float s) {
-  return PLAIN ? fmaf(a, s, h) : apply(Map{a, h}, s);
+#pragma unroll
+  for (int v = 0; v < VEC; v++) m[v].A = chunk_factor(c, m[v].A);
 }
 
 template <bool PLAIN, typename T, int VEC, int K>
-__device__ __forceinline__ void write_states(const Chunk& c, const float (&ca)[K][VEC], const float (&ch)[K][VEC],
-                                             const float (&in)[VEC], T* __restrict__ y, int64_t stride) {
+__device__ __forceinline__ void write_states(const Chunk& c, const float (&aa)[K][VEC], const float (&uu)[K][VEC],
+                                             float (&h)[VEC], T* __restrict__ y, int64_t stride) {
 #pragma unroll
   for (int i = 0; i < K; i++) {
     if (PLAIN || i < c.rows) {
+      const bool drop = !PLAIN && ((c.resets >> i) & 1), has = PLAIN || i < c.cnt;
       float o[VEC];
 #pragma unroll
-      for (int v = 0; v < VEC; v++) o[v] = PLAIN || i < c.cnt ? carry<PLAIN>(ca[i][v], ch[i][v], in[v]) : 0.f;
+      for (int v = 0; v < VEC; v++) {
+        if (has) h[v] = drop ? uu[i][v] : fmaf(aa[i][v], h[v], uu[i][v]);
+        o[v] = has ? h[v] : 0.f;
+      }
       store_vec<T, VEC>(y + i * stride, o);
     }
   }
@@ -208,7 +213,7 @@ __device__ __forceinline__ void write_states(const Chunk& c, const float (&ca)[K
 
 // `per` tiles in a segment.
 template <typename T, int VEC>
-__global__ __launch_bounds__(kScanThreads) void k_scan_fwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
+__global__ __launch_bounds__(kScanThreads, 4) void k_scan_fwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
                                                            T* __restrict__ y, int nseg, int per,
                                                            const Map* __restrict__ seg_maps) {
   constexpr int K = chunk_steps<T>();
@@ -227,16 +232,14 @@ __global__ __launch_bounds__(kScanThreads) void k_scan_fwd(ScanArgs p, const T* 
   float carry[VEC];
   start_state<VEC>(p, s, s.seg, p.h0, seg_maps, carry);
   for (int tile = first; tile < last; tile++) {
-    float ca[K][VEC], ch[K][VEC], in[VEC];
+    float aa[K][VEC], uu[K][VEC], in[VEC];
     Map m[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
     const Chunk now = c;
     const bool plain = now.cnt == K && now.resets == 0;
     if (plain)
-      compose<true, T, VEC, K>(now, xr, gr, ca, ch, m);
+      compose<true, T, VEC, K>(now, xr, gr, aa, uu, m);
     else
-      compose<false, T, VEC, K>(now, xr, gr, ca, ch, m);
+      compose<false, T, VEC, K>(now, xr, gr, aa, uu, m);
     if (tile + 1 < last) {
       c = chunk_of<K>(p, s, n, (tile + 1) * s.waves + s.wave);
       if (live) {
@@ -249,20 +252,22 @@ __global__ __launch_bounds__(kScanThreads) void k_scan_fwd(ScanArgs p, const T* 
     if (now.rows > 0 && p.ckpt) store_vec<float, VEC>(p.ckpt + (s.b * nck + now.ck) * p.D + s.d, in);
     T* yp = y + (s.b * p.L + now.t0) * p.D + s.d;
     if (plain)
-      write_states<true, T, VEC, K>(now, ca, ch, in, yp, p.D);
+      write_states<true, T, VEC, K>(now, aa, uu, in, yp, p.D);
     else
-      write_states<false, T, VEC, K>(now, ca, ch, in, yp, p.D);
+      write_states<false, T, VEC, K>(now, aa, uu, in, yp, p.D);
   }
   if (live && s.wave == 0 && s.seg == nseg - 1) store_vec<float, VEC>(p.h_last + s.b * p.D + s.d, carry);
 }
 
-// One chunk backward: z, the gate's factor dg / dh (cc) and, running against time, the composition of what reaches the
-// state behind step i from outside the chunk (aa) and from inside (dh).
+// One chunk backward: z, 1 - z and the gate's factor dg / dh (cc) of each step, and the chunk's map of the state's
+// gradient. The gradients themselves follow in write_grads, from what enters the chunk.
 template <bool PLAIN, typename T, int VEC, int K>
 __device__ __forceinline__ void compose_back(const Chunk& c, const VecOf<T, VEC> (&x)[K], const VecOf<T, VEC> (&g)[K],
                                              const VecOf<T, VEC> (&dy)[K], bool has_dy, float (&h)[VEC],
-                                             float (&zz)[K][VEC], float (&cc)[K][VEC], float (&aa)[K][VEC],
-                                             float (&dh)[K][VEC], Map (&m)[VEC]) {
+                                             float (&zz)[K][VEC], float (&aa)[K][VEC], float (&cc)[K][VEC],
+                                             Map (&m)[VEC]) {
+#pragma unroll
+  for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
 #pragma unroll
   for (int i = 0; i < K; i++) {
     const bool drop = !PLAIN && ((c.resets >> i) & 1);
@@ -278,34 +283,36 @@ __device__ __forceinline__ void compose_back(const Chunk& c, const VecOf<T, VEC>
   }
 #pragma unroll
   for (int i = K - 1; i >= 0; i--) {
-    const bool drop = !PLAIN && ((c.resets >> i) & 1), dropped = !PLAIN && (c.resets >> i) != 0;
+    const bool drop = !PLAIN && ((c.resets >> i) & 1);
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
       if (PLAIN || i < c.cnt) {
-        const float d = has_dy ? m[v].H + to_f32(dy[i].v[v]) : m[v].H, a = aa[i][v];
-        dh[i][v] = d;
-        aa[i][v] = m[v].A;
-        m[v].H = drop ? 0.f : a * d;
-        m[v].A = dropped ? 0.f : fmaxf(m[v].A * a, kTiny);
+        const float d = has_dy ? m[v].H + to_f32(dy[i].v[v]) : m[v].H;
+        m[v].H = drop ? 0.f : aa[i][v] * d;
+        m[v].A *= aa[i][v];
       }
     }
   }
+#pragma unroll
+  for (int v = 0; v < VEC; v++) m[v].A = chunk_factor(c, m[v].A);
 }
 
 template <bool PLAIN, typename T, int VEC, int K>
-__device__ __forceinline__ void write_grads(const Chunk& c, const float (&zz)[K][VEC], const float (&cc)[K][VEC],
-                                            const float (&aa)[K][VEC], const float (&dh)[K][VEC], const float (&in)[VEC],
-                                            T* __restrict__ dx, T* __restrict__ dg, int64_t stride) {
+__device__ __forceinline__ void write_grads(const Chunk& c, const VecOf<T, VEC> (&dy)[K], bool has_dy,
+                                            const float (&zz)[K][VEC], const float (&aa)[K][VEC],
+                                            const float (&cc)[K][VEC], float (&in)[VEC], T* __restrict__ dx,
+                                            T* __restrict__ dg, int64_t stride) {
 #pragma unroll
-  for (int i = 0; i < K; i++) {
+  for (int i = K - 1; i >= 0; i--) {
     if (PLAIN || i < c.rows) {
+      const bool drop = !PLAIN && ((c.resets >> i) & 1), has = PLAIN || i < c.cnt;
       float ox[VEC], og[VEC];
 #pragma unroll
       for (int v = 0; v < VEC; v++) {
-        const bool has = PLAIN || i < c.cnt;
-        const float d = has ? carry<PLAIN>(aa[i][v], dh[i][v], in[v]) : 0.f;
+        const float d = has_dy && has ? in[v] + to_f32(dy[i].v[v]) : in[v];
         ox[v] = has ? d * zz[i][v] : 0.f;
         og[v] = has ? d * cc[i][v] : 0.f;
+        if (has) in[v] = drop ? 0.f : d * aa[i][v];
       }
       store_vec<T, VEC>(dx + i * stride, ox);
       store_vec<T, VEC>(dg + i * stride, og);
@@ -324,7 +331,7 @@ __global__ __launch_bounds__(kScanThreads) void k_scan_bwd(ScanArgs p, const T* 
   const bool live = s.d < p.D;
   const int n = length_of(p.lengths, s.b, int(p.L)), nck = int((p.L + K - 1) / K);
   const int first = (nseg - 1 - s.seg) * per, last = max(first + 1, min(first + per, (nck + s.waves - 1) / s.waves));
-  const T *xp = x + s.b * p.xsb + s.d, *gp = g + s.b * p.gsb + s.d, *yp = dy + s.b * p.ysb + s.d;
+  const T *xp = x + s.b * p.xsb + s.d, *gp = g + s.b * p.gsb + s.d, *yp = dy ? dy + s.b * p.ysb + s.d : nullptr;
   VecOf<T, VEC> xr[K], gr[K], yr[K];
   float h[VEC] = {};
   Chunk c;
@@ -340,42 +347,75 @@ __global__ __launch_bounds__(kScanThreads) void k_scan_bwd(ScanArgs p, const T* 
   float carry[VEC];
   start_state<VEC>(p, s, s.seg, p.dh_last, seg_maps, carry);
   for (int tile = last - 1; tile >= first; tile--) {
-    float zz[K][VEC], cc[K][VEC], aa[K][VEC], dh[K][VEC], in[VEC];
+    float zz[K][VEC], aa[K][VEC], cc[K][VEC], in[VEC];
+    VecOf<T, VEC> yn[K];
     Map m[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
     const Chunk now = c;
     const bool plain = now.cnt == K && now.resets == 0 && dy != nullptr;
     if (plain)
-      compose_back<true, T, VEC, K>(now, xr, gr, yr, true, h, zz, cc, aa, dh, m);
+      compose_back<true, T, VEC, K>(now, xr, gr, yr, true, h, zz, aa, cc, m);
     else
-      compose_back<false, T, VEC, K>(now, xr, gr, yr, dy != nullptr, h, zz, cc, aa, dh, m);
+      compose_back<false, T, VEC, K>(now, xr, gr, yr, dy != nullptr, h, zz, aa, cc, m);
+#pragma unroll
+    for (int i = 0; i < K; i++) yn[i] = yr[i];
     if (tile > first) load(tile - 1);
     exchange<VEC>(s, false, maps[tile & 1], m, carry, in);
     if (!live) continue;
     T *dxp = dx + s.b * p.dsb + now.t0 * p.dst + s.d, *dgp = dg + s.b * p.dsb + now.t0 * p.dst + s.d;
     if (plain)
-      write_grads<true, T, VEC, K>(now, zz, cc, aa, dh, in, dxp, dgp, p.dst);
+      write_grads<true, T, VEC, K>(now, yn, true, zz, aa, cc, in, dxp, dgp, p.dst);
     else
-      write_grads<false, T, VEC, K>(now, zz, cc, aa, dh, in, dxp, dgp, p.dst);
+      write_grads<false, T, VEC, K>(now, yn, dy != nullptr, zz, aa, cc, in, dxp, dgp, p.dst);
   }
   if (live && p.dh0 && s.wave == 0 && s.seg == nseg - 1) store_vec<float, VEC>(p.dh0 + s.b * p.D + s.d, carry);
 }
 
+// m becomes the chunk's map: forward of (gate, input), backward of (gate, dy).
+template <bool FORWARD, bool PLAIN, typename T, int VEC, int K>
+__device__ __forceinline__ void compose_map(const Chunk& c, const VecOf<T, VEC> (&g)[K], const VecOf<T, VEC> (&in)[K],
+                                            bool has_in, Map (&m)[VEC]) {
+#pragma unroll
+  for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
+#pragma unroll
+  for (int q = 0; q < K; q++) {
+    const int i = FORWARD ? q : K - 1 - q;
+    const bool drop = !PLAIN && ((c.resets >> i) & 1);
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+      if (PLAIN || i < c.cnt) {
+        float z, a;
+        gate_of(to_f32(g[i].v[v]), z, a);
+        const float iv = PLAIN || has_in ? to_f32(in[i].v[v]) : 0.f;
+        if (FORWARD)
+          m[v].H = drop ? z * iv : fmaf(a, m[v].H, z * iv);
+        else
+          m[v].H = drop ? 0.f : a * (m[v].H + iv);
+        m[v].A *= a;
+      }
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < VEC; v++) m[v].A = chunk_factor(c, m[v].A);
+}
+
 // The maps of all segments but the last, in the order of the recurrence: forward of (gate, input), backward of
-// (gate, dy). Each wave composes a run of neighbouring chunks on its own; the runs are joined at the end.
+// (gate, dy). Each wave composes a run of neighbouring chunks on its own; the runs are joined at the end. `len` chunks
+// in a segment. Little is kept from chunk to chunk, so 32 waves a CU hide the loads.
+constexpr int kMapWaves = 16;
+
 template <typename T, int VEC, bool FORWARD>
-__global__ __launch_bounds__(kScanThreads) void k_scan_maps(ScanArgs p, const T* __restrict__ g, const T* __restrict__ in,
-                                                            int nseg, int per, Map* __restrict__ seg_maps) {
+__global__ __launch_bounds__(kMapWaves* kWave, 8) void k_scan_maps(ScanArgs p, const T* __restrict__ g,
+                                                                   const T* __restrict__ in, int nseg, int len,
+                                                                   Map* __restrict__ seg_maps) {
   constexpr int K = chunk_steps<T>();
-  __shared__ Map maps[kScanWaves][kWave * VEC];
+  __shared__ Map maps[kMapWaves][kWave * VEC];
   const ScanPlace s = scan_place<VEC>(p);
   const bool live = s.d < p.D;
   const int n = length_of(p.lengths, s.b, int(p.L)), nck = int((p.L + K - 1) / K);
-  const int seg = FORWARD ? s.seg : nseg - 1 - s.seg;  // in time; a tile has s.waves chunks, so a wave's run has `per`
-  const int lo = seg * per * s.waves + s.wave * per, hi = min(lo + per, nck);
+  const int begin = (FORWARD ? s.seg : nseg - 1 - s.seg) * len, end = min(begin + len, nck);
+  const int each = (len + s.waves - 1) / s.waves, lo = min(begin + s.wave * each, end), hi = min(lo + each, end);
   const int64_t isb = FORWARD ? p.xsb : p.ysb, ist = FORWARD ? p.xst : p.yst;
-  const T *gp = g + s.b * p.gsb + s.d, *ip = in + s.b * isb + s.d;
+  const T *gp = g + s.b * p.gsb + s.d, *ip = in ? in + s.b * isb + s.d : nullptr;
   Map m[VEC];
 #pragma unroll
   for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
@@ -385,24 +425,13 @@ __global__ __launch_bounds__(kScanThreads) void k_scan_maps(ScanArgs p, const T*
     VecOf<T, VEC> gr[K], ir[K];
     load_rows<T, VEC, K>(gp + c.t0 * p.gst, p.gst, c.cnt, gr);
     if (in) load_rows<T, VEC, K>(ip + c.t0 * ist, ist, c.cnt, ir);
+    Map cm[VEC];
+    if (c.cnt == K && c.resets == 0 && in)
+      compose_map<FORWARD, true, T, VEC, K>(c, gr, ir, true, cm);
+    else
+      compose_map<FORWARD, false, T, VEC, K>(c, gr, ir, in != nullptr, cm);
 #pragma unroll
-    for (int q = 0; q < K; q++) {
-      const int i = FORWARD ? q : K - 1 - q;
-      const bool drop = (c.resets >> i) & 1;
-#pragma unroll
-      for (int v = 0; v < VEC; v++) {
-        if (i < c.cnt) {
-          float z, a;
-          gate_of(to_f32(gr[i].v[v]), z, a);
-          const float iv = in ? to_f32(ir[i].v[v]) : 0.f;
-          if (FORWARD)
-            m[v].H = drop ? z * iv : fmaf(a, m[v].H, z * iv);
-          else
-            m[v].H = drop ? 0.f : a * (m[v].H + iv);
-          m[v].A = drop || m[v].A == 0.f ? 0.f : fmaxf(m[v].A * a, kTiny);
-        }
-      }
-    }
+    for (int v = 0; v < VEC; v++) m[v] = then(m[v], cm[v]);
   }
 #pragma unroll
   for (int v = 0; v < VEC; v++) maps[s.wave][s.lane * VEC + v] = m[v];
@@ -471,8 +500,8 @@ void scan_fwd_t(const ScanArgs& p, const T* x, const T* g, T* y, int type, hipSt
   const dim3 block(uint32_t(s.waves * kWave));
   if (s.nseg > 1) {
     if (maps == nullptr) throw std::invalid_argument("gated_scan: no workspace");
-    hipLaunchKernelGGL((k_scan_maps<T, VEC, true>), dim3(uint32_t(s.chains * (s.nseg - 1))), block, 0, stream, p, g, x,
-                       s.nseg, s.per, maps);
+    hipLaunchKernelGGL((k_scan_maps<T, VEC, true>), dim3(uint32_t(s.chains * (s.nseg - 1))), dim3(kMapWaves * kWave), 0,
+                       stream, p, g, x, s.nseg, s.per * s.waves, maps);
   }
   hipLaunchKernelGGL((k_scan_fwd<T, VEC>), dim3(uint32_t(s.chains * s.nseg)), block, 0, stream, p, x, g, y, s.nseg, s.per,
                      maps);
@@ -486,8 +515,8 @@ void scan_bwd_t(const ScanArgs& p, const T* x, const T* g, const T* dy, T* dx, T
   const dim3 block(uint32_t(s.waves * kWave));
   if (s.nseg > 1) {
     if (maps == nullptr) throw std::invalid_argument("gated_scan backward: no workspace");
-    hipLaunchKernelGGL((k_scan_maps<T, VEC, false>), dim3(uint32_t(s.chains * (s.nseg - 1))), block, 0, stream, p, g, dy,
-                       s.nseg, s.per, maps);
+    hipLaunchKernelGGL((k_scan_maps<T, VEC, false>), dim3(uint32_t(s.chains * (s.nseg - 1))), dim3(kMapWaves * kWave), 0,
+                       stream, p, g, dy, s.nseg, s.per * s.waves, maps);
   }
   hipLaunchKernelGGL((k_scan_bwd<T, VEC>), dim3(uint32_t(s.chains * s.nseg)), block, 0, stream, p, x, g, dy, dx, dg, s.nseg,
                      s.per, maps);

@@ -467,8 +467,11 @@ struct ScanPlan {
 
 int steps_of(int type) { return type == kF32 ? chunk_steps<float>() : chunk_steps<f16_t>(); }
 
-// Workgroups that the passes want before they cut no chain, and that they cut towards.
-constexpr int64_t kEnoughChains = 160, kWantGroups = 512;
+// From kEnoughChains on no chain is cut; with fewer, they are cut into at most kGroups workgroups, one a CU (more would
+// leave a second round of the backward pass to few). Measured on bf16 (us, forward / backward): 104 chains of 4096 steps
+// 110 / 189 cut and 127 / 211 whole, 136 chains 145 / 261 cut and 129 / 214 whole; 8 chains of 65536 steps 127 / 197 in 256
+// segments' workgroups, 127 / 220 in 512, 145 / 250 in 1024.
+constexpr int64_t kEnoughChains = 128, kGroups = 256;
 
 ScanPlan scan_plan(const ScanArgs& p, int type, int vec, const char* who) {
   if (p.L >= (int64_t(1) << 31) - 4096) throw std::invalid_argument(std::string(who) + ": too many steps");
@@ -478,7 +481,7 @@ ScanPlan scan_plan(const ScanArgs& p, int type, int vec, const char* who) {
   const int64_t tiles = (chunks + s.waves - 1) / s.waves, cols = (p.D + kWave * vec - 1) / (kWave * vec);
   if (p.B > (int64_t(1) << 31) / cols / 1024) throw std::invalid_argument(std::string(who) + ": too many sequences");
   s.chains = p.B * cols;
-  int64_t nseg = s.chains >= kEnoughChains ? 1 : std::min(tiles, (kWantGroups + s.chains - 1) / s.chains);
+  int64_t nseg = s.chains >= kEnoughChains ? 1 : std::min(tiles, kGroups / s.chains);
   s.per = int((tiles + nseg - 1) / nseg);
   s.nseg = int((tiles + s.per - 1) / s.per);
   return s;

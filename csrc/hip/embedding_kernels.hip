@@ -155,25 +155,25 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(const TI* __restri
   }
 }
 
-constexpr int kSortThreads = 256, kSortWaves = kSortThreads / kWave, kMaxBits = 9, kMaxRadix = 1 << kMaxBits;
-constexpr int kMaxTiles = 256, kMinTile = 1024;
+constexpr int kHistThreads = 256, kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
+constexpr int kMaxBits = 9, kMaxRadix = 1 << kMaxBits, kMaxTiles = 256;
 
 // Digit counts of each tile: counts[tile][radix].
 template <typename TI>
-__global__ __launch_bounds__(kSortThreads) void k_sort_hist(const TI* __restrict__ ids, const uint32_t* __restrict__ keys,
+__global__ __launch_bounds__(kHistThreads) void k_sort_hist(const TI* __restrict__ ids, const uint32_t* __restrict__ keys,
                                                             int64_t n, int64_t tile, int64_t V, int64_t pad, int shift,
                                                             int bits, uint32_t* __restrict__ counts) {
   __shared__ uint32_t hist[kMaxRadix];
   const int radix = 1 << bits;
-  for (int r = threadIdx.x; r < radix; r += kSortThreads) hist[r] = 0;
+  for (int r = threadIdx.x; r < radix; r += kHistThreads) hist[r] = 0;
   __syncthreads();
   const int64_t lo = int64_t(blockIdx.x) * tile, hi = min(n, lo + tile);
-  for (int64_t i = lo + threadIdx.x; i < hi; i += kSortThreads) {
+  for (int64_t i = lo + threadIdx.x; i < hi; i += kHistThreads) {
     const uint32_t k = ids ? embed_key(ids[i], V, pad) : keys[i];
     atomicAdd(&hist[(k >> shift) & (radix - 1)], 1u);
   }
   __syncthreads();
-  for (int r = threadIdx.x; r < radix; r += kSortThreads) counts[int64_t(blockIdx.x) * radix + r] = hist[r];
+  for (int r = threadIdx.x; r < radix; r += kHistThreads) counts[int64_t(blockIdx.x) * radix + r] = hist[r];
 }
 
 // One stable pass: tile after tile, wave after wave, round after round, lane after lane is the input order,
@@ -187,6 +187,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(const TI* __restr
                                                                uint32_t* __restrict__ okeys, uint32_t* __restrict__ opos) {
   __shared__ uint32_t base[kMaxRadix];               // slot of the digit's first element of this tile
   __shared__ uint32_t slot[kSortWaves][kMaxRadix];   // counts, then running slots, of each wave
+  __shared__ uint4 part[4][kMaxRadix / 2];
   __shared__ uint32_t wsum[kSortWaves];
   const int radix = 1 << bits, tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
   const int64_t lo = int64_t(blockIdx.x) * tile, hi = min(n, lo + tile);
@@ -197,39 +198,48 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(const TI* __restr
     const uint32_t k = ids ? embed_key(ids[i], V, pad) : keys[i];
     atomicAdd(&slot[wave][(k >> shift) & (radix - 1)], 1u);
   }
-  // digits 2t and 2t+1 belong to thread t: totals over all tiles, and the part of the earlier tiles
-  const int r0 = 2 * tid;
+  // digit totals over all tiles, and the part of the tiles before this one: two digits a thread, and the tiles dealt out
+  // to four groups of threads
+  const int pair = tid % (kMaxRadix / 2), quarter = tid / (kMaxRadix / 2), r0 = 2 * pair;
   uint32_t total[2] = {0, 0}, before[2] = {0, 0};
   if (r0 < radix) {
     const uint2* col = reinterpret_cast<const uint2*>(counts + r0);  // radix is even: bits >= 1
     const int tiles = int(gridDim.x), mine = int(blockIdx.x);
-    int b = 0;
-    for (; b + 8 <= tiles; b += 8) {
+    for (int b0 = quarter; b0 < tiles; b0 += 4 * 8) {
       uint2 c[8];
 #pragma unroll
-      for (int k = 0; k < 8; k++) c[k] = col[int64_t(b + k) * (radix / 2)];
+      for (int k = 0; k < 8; k++) {
+        const int b = b0 + 4 * k;
+        c[k] = col[int64_t(b < tiles ? b : 0) * (radix / 2)];
+      }
 #pragma unroll
       for (int k = 0; k < 8; k++) {
-        total[0] += c[k].x, total[1] += c[k].y;
-        if (b + k < mine) before[0] += c[k].x, before[1] += c[k].y;
+        const int b = b0 + 4 * k;
+        if (b < tiles) total[0] += c[k].x, total[1] += c[k].y;
+        if (b < mine) before[0] += c[k].x, before[1] += c[k].y;
       }
     }
-    for (; b < tiles; b++) {
-      const uint2 c = col[int64_t(b) * (radix / 2)];
-      total[0] += c.x, total[1] += c.y;
-      if (b < mine) before[0] += c.x, before[1] += c.y;
-    }
   }
-  uint32_t incl = total[0] + total[1];
-  for (int off = 1; off < kWave; off <<= 1) {
-    const uint32_t up = __shfl_up(incl, off);
-    if (lane >= off) incl += up;
-  }
-  if (lane == kWave - 1) wsum[wave] = incl;
+  part[quarter][pair] = uint4{total[0], total[1], before[0], before[1]};
   __syncthreads();
-  uint32_t excl = incl - total[0] - total[1];
-  for (int w = 0; w < wave; w++) excl += wsum[w];
-  if (r0 < radix) {
+  // exclusive sums of the totals in the order of the digits, by the first group
+  uint32_t incl = 0;
+  if (quarter == 0) {
+    for (int q = 1; q < 4; q++) {
+      const uint4 o = part[q][pair];
+      total[0] += o.x, total[1] += o.y, before[0] += o.z, before[1] += o.w;
+    }
+    incl = total[0] + total[1];
+    for (int off = 1; off < kWave; off <<= 1) {
+      const uint32_t up = __shfl_up(incl, off);
+      if (lane >= off) incl += up;
+    }
+    if (lane == kWave - 1) wsum[wave] = incl;
+  }
+  __syncthreads();
+  if (quarter == 0 && r0 < radix) {
+    uint32_t excl = incl - total[0] - total[1];
+    for (int w = 0; w < wave; w++) excl += wsum[w];
     base[r0] = excl + before[0];
     base[r0 + 1] = excl + total[0] + before[1];
   }
@@ -352,13 +362,15 @@ __global__ __launch_bounds__(256) void k_embed_sum(const uint32_t* __restrict__ 
     write_row<TW, VEC>(dw, int64_t(cur) * D + c, acc, scale);
 }
 
-// A workgroup per piece and chunk: the row whose segment starts in piece p and goes on behind it. The four waves add
-// up consecutive quarters of the pieces it covers; the quarters are joined in order.
+// A workgroup per piece and chunk: the row whose segment starts in piece p and goes on behind it. The waves add up
+// consecutive runs of the pieces it covers; the runs are joined in order.
+constexpr int kJoinWaves = 8;
+
 template <typename TW, int VEC>
-__global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__ keys, uint32_t n,
+__global__ __launch_bounds__(kJoinWaves* kWave) void k_embed_join(const uint32_t* __restrict__ keys, uint32_t n,
                                                     const float* __restrict__ part, TW* __restrict__ dw, int64_t V,
                                                     int64_t D, float scale, SumPlan s) {
-  __shared__ float quarter[4][kWave * VEC];
+  __shared__ float run[kJoinWaves][kWave * VEC];
   const int64_t p = blockIdx.x / s.chunks, ch = blockIdx.x - p * s.chunks;
   const uint32_t lo = uint32_t(p * s.piece), hi = uint32_t(min(int64_t(n), int64_t(lo) + s.piece));
   if (hi >= n) return;
@@ -374,11 +386,11 @@ __global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__
   }
   const int64_t c = ((ch << s.lpr) + lane) * VEC;
   const bool live = lane < (1 << s.lpr) && c < D;
-  const int64_t per = (count + 3) / 4, q0 = min(count, wave * per), q1 = min(count, q0 + per);
+  const int64_t per = (count + kJoinWaves - 1) / kJoinWaves, q0 = min(count, wave * per), q1 = min(count, q0 + per);
   float acc[VEC] = {};
   if (live) {
     // piece p left its sum in slot 2p + 1, the pieces p + 1, p + 2, .. in slots 2p + 2, 2p + 4, ..
-#pragma unroll 8
+#pragma unroll 16
     for (int64_t q = q0; q < q1; q++) {
       float x[VEC];
       load_vec<float, VEC>(part + (2 * (p + q) + (q == 0 ? 1 : 0)) * D + c, x);
@@ -387,13 +399,13 @@ __global__ __launch_bounds__(256) void k_embed_join(const uint32_t* __restrict__
     }
   }
 #pragma unroll
-  for (int e = 0; e < VEC; e++) quarter[wave][lane * VEC + e] = acc[e];
+  for (int e = 0; e < VEC; e++) run[wave][lane * VEC + e] = acc[e];
   __syncthreads();
   if (wave == 0 && live) {
 #pragma unroll
-    for (int w = 1; w < 4; w++)
+    for (int w = 1; w < kJoinWaves; w++)
 #pragma unroll
-      for (int e = 0; e < VEC; e++) acc[e] += quarter[w][lane * VEC + e];
+      for (int e = 0; e < VEC; e++) acc[e] += run[w][lane * VEC + e];
     write_row<TW, VEC>(dw, int64_t(v) * D + c, acc, scale);
   }
 }
@@ -425,20 +437,21 @@ SortPlan sort_plan(int64_t n, int64_t V) {
   p.passes = (nb + most - 1) / most;
   p.bits = (nb + p.passes - 1) / p.passes;
   const int64_t per = (n + kMaxTiles - 1) / kMaxTiles;
-  p.tile = std::max<int64_t>(kMinTile, (per + kSortThreads - 1) / kSortThreads * kSortThreads);
+  p.tile = std::max<int64_t>(1, (per + kSortThreads - 1) / kSortThreads) * kSortThreads;
   p.tiles = int((n + p.tile - 1) / p.tile);
   return p;
 }
 
-// Pieces of 16 to 128 positions: short enough that about 3000 waves walk them, long enough that the sums left between
-// pieces (8 bytes a column and piece, written and read) stay below the rows themselves.
-SumPlan sum_plan(int64_t n, int64_t D, int vec) {
+// Pieces of 16 to 256 positions: short enough that about 1500 waves walk them (twice as many where a lane has less than
+// 16 bytes of a row), long enough that the sums left between pieces (8 bytes a column and piece, written and read) stay
+// below the rows themselves. 131072 rows of 1024 bytes on two tokens take 96 us so, and 153 in twice as many pieces.
+SumPlan sum_plan(int64_t n, int64_t D, int vec, bool wide) {
   SumPlan s;
   s.lpr = std::min(6, lanes_log2(D, vec));
   s.chunks = (D + (int64_t(vec) << s.lpr) - 1) / (int64_t(vec) << s.lpr);
-  const int64_t lanes = s.chunks << s.lpr;
+  const int64_t lanes = s.chunks << s.lpr, waves = wide ? 1536 : 3072;
   s.piece = 16;
-  while (s.piece < 128 && n / (2 * s.piece) * lanes >= 3072 * kWave) s.piece *= 2;
+  while (s.piece < 256 && n / (2 * s.piece) * lanes >= waves * kWave) s.piece *= 2;
   s.pieces = (n + s.piece - 1) / s.piece;
   return s;
 }
@@ -477,7 +490,7 @@ void embed_sort(const TI* ids, int64_t n, int64_t V, int64_t pad, uint32_t* ws, 
   uint32_t* counts = ws + (4 * n + 1) / 2 * 2;  // read in pairs
   for (int s = 0; s < p.passes && !p.small; s++) {
     const TI* src = s == 0 ? ids : nullptr;
-    hipLaunchKernelGGL((k_sort_hist<TI>), dim3(p.tiles), dim3(kSortThreads), 0, stream, src, kin, n, p.tile, V, pad,
+    hipLaunchKernelGGL((k_sort_hist<TI>), dim3(p.tiles), dim3(kHistThreads), 0, stream, src, kin, n, p.tile, V, pad,
                        s * p.bits, p.bits, counts);
     hipLaunchKernelGGL((k_sort_scatter<TI>), dim3(p.tiles), dim3(kSortThreads), 0, stream, src, kin, pin, n, p.tile, V,
                        pad, s * p.bits, p.bits, counts, buf[s & 1][0], buf[s & 1][1]);
@@ -497,14 +510,14 @@ int64_t sort_words(int64_t n, int64_t V) {
 template <typename TW, typename TO, int VEC>
 void embed_sum_t(const uint32_t* keys, const uint32_t* pos, int64_t n, const TO* dy, int64_t dys, TW* dw, float* part,
                  int64_t V, int64_t D, float scale, hipStream_t stream) {
-  const SumPlan s = sum_plan(n, D, VEC);
+  const SumPlan s = sum_plan(n, D, VEC, VEC * sizeof(TO) >= 16);
   const int64_t sums = ((s.pieces * s.chunks << s.lpr) + 255) / 256, zeros = (V + kZeroRows - 1) / kZeroRows;
   if (sums + zeros > (int64_t(1) << 31) - 1) throw std::invalid_argument("embedding_grad: too many elements");
   hipLaunchKernelGGL((k_embed_sum<TW, TO, VEC>), dim3(uint32_t(sums + zeros)), dim3(256), 0, stream, keys, pos,
                      uint32_t(n), dy, dys, dw, part, V, D, scale, s, uint32_t(sums));
   if (s.pieces > 1)
-    hipLaunchKernelGGL((k_embed_join<TW, VEC>), dim3(uint32_t(s.pieces * s.chunks)), dim3(256), 0, stream, keys,
-                       uint32_t(n), part, dw, V, D, scale, s);
+    hipLaunchKernelGGL((k_embed_join<TW, VEC>), dim3(uint32_t(s.pieces * s.chunks)), dim3(kJoinWaves * kWave), 0,
+                       stream, keys, uint32_t(n), part, dw, V, D, scale, s);
   RMM_HIP_CHECK(hipGetLastError());
 }
 

@@ -20,7 +20,7 @@ from ray_memory_management_amd.tune.trainable import Trainable
 
 class Algorithm(Trainable):
     _config_class = AlgorithmConfig
-    # model["use_lstm"] / model["use_attention"]: only algorithms whose learners train sequence
+    # model["use_lstm"] / model["use_gated_scan"] / model["use_attention"]: only algorithms whose learners train sequence
     # models accept them (PPO, IMPALA / APPO; R2D2 brings its own recurrent Q-model); everywhere
     # else they raise instead of being silently ignored
     _supports_sequence_models = False
@@ -50,7 +50,7 @@ class Algorithm(Trainable):
 
         if wants_sequence_model(c.model) and not self._supports_sequence_models:
             raise ValueError(f"{type(self).__name__} does not train recurrent / attention models: model config "
-                             f"use_lstm / use_attention is supported by PPO, IMPALA and APPO (R2D2 for recurrent "
+                             f"use_lstm / use_gated_scan / use_attention is supported by PPO, IMPALA and APPO (R2D2 for recurrent "
                              f"Q-learning)")
         env_creator = c.env if callable(c.env) and not isinstance(c.env, str) else None
         cfg = c.to_dict()

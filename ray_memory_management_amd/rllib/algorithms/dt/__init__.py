@@ -8,8 +8,11 @@ episodes, left-padded with an attention mask, returns-to-go per step), dt_torch_
 (R̂_t, s_t, a_t) + timestep embeddings → causal GPT → action predicted from the state token) and
 dt_torch_policy.py (evaluation: condition on the target return, subtract each reward).
 
-On MI355X the transformer is plain torch (SDPA attention, bf16 autocast on the GPU); the episode
-store is columnar numpy and a training batch is one fancy-index gather per column.
+On MI355X the transformer is plain torch (SDPA attention, bf16 autocast on the GPU); timesteps and
+actions are looked up with ``ops.Embedding`` (gradients by sorted ids). ``counter_dropout`` drops the
+token embeddings with ``ops.Dropout``, whose masks follow from the seed and the step alone: the same
+on the CPU and the GPU, and none is stored. The episode store is columnar numpy and a training batch
+is one fancy-index gather per column.
 """
 from __future__ import annotations
 
@@ -20,6 +23,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 
+from ray_memory_management_amd import ops
 from ray_memory_management_amd.rllib.algorithms.algorithm import Algorithm
 from ray_memory_management_amd.rllib.algorithms.algorithm_config import AlgorithmConfig
 from ray_memory_management_amd.rllib.env import make_env
@@ -37,6 +41,7 @@ class DTConfig(AlgorithmConfig):
         self.embed_pdrop = 0.1
         self.resid_pdrop = 0.1
         self.attn_pdrop = 0.1
+        self.counter_dropout = False
         self.max_seq_len = 5
         self.lr = 1e-4
         self.lr_warmup_steps = 0
@@ -51,15 +56,15 @@ class DTConfig(AlgorithmConfig):
 
 class DTModel(nn.Module):
     def __init__(self, obs_dim: int, num_actions: int, K: int, horizon: int, E: int, layers: int, heads: int,
-                 pdrop: float, attn_pdrop: float):
+                 pdrop: float, attn_pdrop: float, counter_dropout: bool = False, seed: int = 0):
         super().__init__()
         self.K, self.E, self.A = K, E, num_actions
-        self.embed_t = nn.Embedding(horizon + 1, E)
+        self.embed_t = ops.Embedding(horizon + 1, E)
         self.embed_r = nn.Linear(1, E)
         self.embed_s = nn.Linear(obs_dim, E)
-        self.embed_a = nn.Embedding(num_actions + 1, E)  # last id = padding / unknown action
+        self.embed_a = ops.Embedding(num_actions + 1, E)  # last id = padding / unknown action
         self.ln = nn.LayerNorm(E)
-        self.drop = nn.Dropout(pdrop)
+        self.drop = ops.Dropout(pdrop, seed) if counter_dropout else nn.Dropout(pdrop)
         layer = nn.TransformerEncoderLayer(E, heads, 4 * E, dropout=attn_pdrop, activation="gelu", batch_first=True,
                                            norm_first=True)
         self.gpt = nn.TransformerEncoder(layer, layers)
@@ -135,7 +140,7 @@ class DT(Algorithm):
         if c.seed is not None:
             torch.manual_seed(int(c.seed))
         self.model = DTModel(obs_dim, env.action_space.n, c.max_seq_len, self.horizon, c.embed_dim, c.num_layers,
-                             c.num_heads, c.embed_pdrop, c.attn_pdrop).to(self.device)
+                             c.num_heads, c.embed_pdrop, c.attn_pdrop, c.counter_dropout, int(c.seed or 0)).to(self.device)
         allobs = np.concatenate([e["obs"].reshape(len(e["obs"]), -1) for e in self.episodes]).astype(np.float64)
         self.model.obs_mean.copy_(torch.as_tensor(allobs.mean(0), dtype=torch.float32))
         self.model.obs_std.copy_(torch.as_tensor(allobs.std(0) + 1e-6, dtype=torch.float32))

@@ -84,7 +84,7 @@ class PPO(Algorithm):
                 raise ValueError(f"{type(self).__name__} does not train recurrent / attention models")
             if getattr(c, "gpu_rollouts", False):
                 raise ValueError("gpu_rollouts (device env + fused sampler) runs feed-forward policies only; "
-                                 "use CPU rollout workers with use_lstm / use_attention")
+                                 "use CPU rollout workers with use_lstm / use_gated_scan / use_attention")
             # sequences need the state recorded by the rollout: GAE + sequence layout on the workers
             c.postprocess_on_learner = False
         if c.num_learner_workers and c.num_learner_workers > 1:

@@ -10,6 +10,7 @@ from typing import Callable, List, Optional
 
 import ray_memory_management_amd as ray
 from ray_memory_management_amd.rllib.evaluation.rollout_worker import RolloutWorker
+from ray_memory_management_amd.rllib.recurrent_net import wants_sequence_model
 from ray_memory_management_amd.rllib.sample_batch import SampleBatch, concat_samples
 
 
@@ -32,8 +33,8 @@ class WorkerSet:
             from ray_memory_management_amd.rllib.evaluation.gpu_rollout_worker import GPURolloutWorker
 
             cls = GPURolloutWorker
-        elif self._config.get("num_gpus_per_worker", 0) and env_creator is None and not (
-                (self._config.get("model") or {}).get("use_lstm") or (self._config.get("model") or {}).get("use_attention")):
+        elif self._config.get("num_gpus_per_worker", 0) and env_creator is None and not wants_sequence_model(
+                self._config.get("model")):
             from ray_memory_management_amd.rllib.env import _VECTOR_REGISTRY
 
             env = self._config.get("env")

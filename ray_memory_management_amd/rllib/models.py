@@ -650,7 +650,7 @@ def build_model(obs_space, action_space, model_config=None) -> nn.Module:
 
     if model_config.get("custom_model"):  # a registered ModelV2 (ModelCatalog), behind (logits, value)
         if wants_sequence_model(model_config):
-            raise ValueError("use_lstm / use_attention wrap the built-in networks; a custom_model must implement "
+            raise ValueError("use_lstm / use_gated_scan / use_attention wrap the built-in networks; a custom_model must implement "
                              "its own memory (ModelV2 state) instead")
         from ray_memory_management_amd.rllib.modelv2 import build_custom_model
 
@@ -688,7 +688,7 @@ from ray_memory_management_amd.rllib.modelv2 import (  # noqa: E402,F401
 # sequence / composite-input networks (reference rllib/models/torch/{recurrent_net,attention_net,
 # complex_input_net}.py)
 from ray_memory_management_amd.rllib.recurrent_net import (  # noqa: E402,F401
-    GTrXLNet, LSTMWrapper, SeqNet as RecurrentNetwork)
+    GatedScanWrapper, GTrXLNet, LSTMWrapper, SeqNet as RecurrentNetwork)
 from ray_memory_management_amd.rllib.complex_input_net import ComplexInputNetwork  # noqa: E402,F401
 
 AttentionWrapper = GTrXLNet

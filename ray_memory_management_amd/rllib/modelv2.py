@@ -39,6 +39,11 @@ MODEL_DEFAULTS: Dict[str, Any] = {
     "lstm_use_prev_action": False,
     "lstm_use_prev_reward": False,
     "_time_major": False,
+    "use_gated_scan": False,
+    "gated_scan_cell_size": 256,
+    "gated_scan_num_layers": 1,
+    "gated_scan_use_prev_action": False,
+    "gated_scan_use_prev_reward": False,
     "use_attention": False,
     "attention_num_transformer_units": 1,
     "attention_dim": 64,

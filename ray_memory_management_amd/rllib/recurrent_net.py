@@ -1,4 +1,4 @@
-"""Sequence models for RLlib policies: the LSTM wrapper and the GTrXL attention wrapper.
+"""Sequence models for RLlib policies: the LSTM, gated-scan and GTrXL attention wrappers.
 
 Parity: reference rllib/models/torch/recurrent_net.py:116 (LSTMWrapper: a memory on top of the
 default network's features, ``lstm_cell_size``, ``lstm_use_prev_action`` / ``lstm_use_prev_reward``,
@@ -7,6 +7,10 @@ default network's features, ``lstm_cell_size``, ``lstm_use_prev_action`` / ``lst
 per-unit memory of past unit inputs) and :260 (AttentionWrapper: GTrXL on top of the default
 network's features plus previous actions / rewards), rllib/models/catalog.py:492-519 (wrapping when
 ``use_lstm`` / ``use_attention`` is set).
+
+``use_gated_scan`` puts layers of a gated linear recurrence (ops.gated_scan) in the LSTM's place. Its
+gates depend on the inputs alone, so a training sequence is one scan with the episode ends as resets,
+where the LSTM steps through every sequence that has one.
 
 Design (framework-native, not the reference's ragged layout): training sequences have ONE fixed
 length ``L = max_seq_len``. A rollout fragment of T steps per env is cut into ceil(T / L) sequences
@@ -31,6 +35,8 @@ from typing import Dict, List, Optional
 import numpy as np
 import torch
 import torch.nn as nn
+
+from ray_memory_management_amd import ops
 
 
 def _act(name):
@@ -180,6 +186,56 @@ class LSTMWrapper(SeqNet):
             y = torch.cat(ys, dim=1)
             hn, cn = h[0], c[0]
         return self.logits(y), self.value(y).squeeze(-1), [hn, cn]
+
+
+# ------------------------------------------------------------------------------------------ gated scan
+class GatedScanWrapper(SeqNet):
+    """Layers of ``h_t = (1 - z_t) h_{t-1} + z_t x_t`` over the trunk features, with x and the gate z both linear in the
+    layer's input (Feng et al. 2024, minGRU); layers after the first add their input. Then the logits and value
+    branches as with the LSTM. State = one [B, cell] fp32 tensor a layer."""
+
+    def __init__(self, obs_space, action_space, num_outputs: int, cfg: Dict):
+        super().__init__(obs_space, action_space, num_outputs, cfg, cfg.get("gated_scan_use_prev_action", False),
+                         cfg.get("gated_scan_use_prev_reward", False))
+        self.cell = int(cfg.get("gated_scan_cell_size", 256))
+        n = int(cfg.get("gated_scan_num_layers", 1))
+        if n < 1:
+            raise ValueError("gated_scan_num_layers must be at least 1")
+        self.layers = nn.ModuleList([nn.Linear(self.cell if i else self.in_dim, 2 * self.cell) for i in range(n)])
+        self.logits = nn.Linear(self.cell, self.num_outputs)
+        self.value = nn.Linear(self.cell, 1)
+        nn.init.orthogonal_(self.logits.weight, 0.01)
+        nn.init.zeros_(self.logits.bias)
+
+    def initial_state(self, batch: int, device=None):
+        dev = device if device is not None else self.logits.weight.device
+        return [torch.zeros(batch, self.cell, device=dev) for _ in self.layers]
+
+    def _out(self, y, state):
+        return self.logits(y), self.value(y).squeeze(-1), state
+
+    def step(self, obs, state, prev_a=None, prev_r=None):
+        x = self._encode(obs, prev_a, prev_r)
+        if torch.is_grad_enabled():
+            y, new = self._scan(x.unsqueeze(1), state, None)
+            return self._out(y[:, 0], new)
+        new = []
+        for i, (proj, h) in enumerate(zip(self.layers, state)):
+            y, h = ops.gated_scan_step(proj(x), None, h.float().contiguous())
+            new.append(h)
+            x = x + y if i else y
+        return self._out(x, new)
+
+    def _scan(self, x, state, resets):
+        new = []
+        for i, (proj, h) in enumerate(zip(self.layers, state)):
+            y, h = ops.gated_scan(proj(x), h0=h, resets=resets)
+            new.append(h)
+            x = x + y if i else y
+        return x, new
+
+    def seq(self, obs, state_in, resets, prev_a=None, prev_r=None):
+        return self._out(*self._scan(self._encode_seq(obs, prev_a, prev_r), state_in, resets))
 
 
 # ------------------------------------------------------------------------------------------ GTrXL
@@ -352,16 +408,22 @@ class GTrXLNet(SeqNet):
 
 
 # ------------------------------------------------------------------------------------------ catalog
+SEQUENCE_KEYS = ("use_lstm", "use_gated_scan", "use_attention")
+
+
 def wants_sequence_model(cfg: Optional[Dict]) -> bool:
     cfg = cfg or {}
-    return bool(cfg.get("use_lstm") or cfg.get("use_attention"))
+    return any(bool(cfg.get(k)) for k in SEQUENCE_KEYS)
 
 
 def build_sequence_model(obs_space, action_space, num_outputs: int, cfg: Dict) -> SeqNet:
-    """reference rllib/models/catalog.py:492-519: wrap the default network in an LSTM or attention
-    memory when the model config asks for one (not both)."""
-    if cfg.get("use_lstm") and cfg.get("use_attention"):
-        raise ValueError("use_lstm and use_attention are mutually exclusive")
+    """reference rllib/models/catalog.py:492-519: wrap the default network in an LSTM, gated-scan or attention
+    memory when the model config asks for one (and only one)."""
+    asked = [k for k in SEQUENCE_KEYS if cfg.get(k)]
+    if len(asked) > 1:
+        raise ValueError(f"{' and '.join(asked)} are mutually exclusive")
+    if cfg.get("use_gated_scan"):
+        return GatedScanWrapper(obs_space, action_space, num_outputs, cfg)
     if cfg.get("use_attention"):
         return GTrXLNet(obs_space, action_space, num_outputs, cfg)
     return LSTMWrapper(obs_space, action_space, num_outputs, cfg)

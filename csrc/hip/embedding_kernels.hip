@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <stdexcept>
+#include <type_traits>
 
 #include "common.h"
 #include "kernels.h"
@@ -461,17 +462,17 @@ void embed_fwd_t(const TI* ids, const void* w, int64_t ws, void* out, int64_t n,
                  hipStream_t stream) {
   const TW* wp = static_cast<const TW*>(w);
   TO* op = static_cast<TO*>(out);
-  constexpr int VEC = 8;
-  const bool wide = D % VEC == 0 && ws % VEC == 0 && vec_aligned<TW, VEC>(w) && vec_aligned<TO, VEC>(out);
-  const int lpr = lanes_log2(D, wide ? VEC : 1);
-  const uint32_t blocks = row_blocks(n, lpr, "embedding");
-  if (wide)
-    hipLaunchKernelGGL((k_embed_fwd<TI, TW, TO, VEC>), dim3(blocks), dim3(256), 0, stream, ids, wp, ws, op, n, V, D,
-                       scale, lpr);
-  else
-    hipLaunchKernelGGL((k_embed_fwd<TI, TW, TO, 1>), dim3(blocks), dim3(256), 0, stream, ids, wp, ws, op, n, V, D,
-                       scale, lpr);
-  RMM_HIP_CHECK(hipGetLastError());
+  const auto run = [&](auto width) {
+    constexpr int VEC = decltype(width)::value;
+    if (D % VEC || ws % VEC || !vec_aligned<TW, VEC>(w) || !vec_aligned<TO, VEC>(out)) return false;
+    const int lpr = lanes_log2(D, VEC);
+    hipLaunchKernelGGL((k_embed_fwd<TI, TW, TO, VEC>), dim3(row_blocks(n, lpr, "embedding")), dim3(256), 0, stream, ids,
+                       wp, ws, op, n, V, D, scale, lpr);
+    RMM_HIP_CHECK(hipGetLastError());
+    return true;
+  };
+  using std::integral_constant;  // the widest rows that the sizes and addresses allow
+  run(integral_constant<int, 8>{}) || run(integral_constant<int, 2>{}) || run(integral_constant<int, 1>{});
 }
 
 template <typename TI>

@@ -479,7 +479,7 @@ ScanPlan scan_plan(const ScanArgs& p, int type, int vec, const char* who) {
   const int64_t chunks = std::max<int64_t>(1, (p.L + steps_of(type) - 1) / steps_of(type));
   s.waves = int(std::min<int64_t>(kScanWaves, chunks));
   const int64_t tiles = (chunks + s.waves - 1) / s.waves, cols = (p.D + kWave * vec - 1) / (kWave * vec);
-  if (p.B > (int64_t(1) << 31) / cols / 1024) throw std::invalid_argument(std::string(who) + ": too many sequences");
+  if (p.B > ((int64_t(1) << 31) - 1) / cols) throw std::invalid_argument(std::string(who) + ": too many sequences");
   s.chains = p.B * cols;
   int64_t nseg = s.chains >= kEnoughChains ? 1 : std::min(tiles, kGroups / s.chains);
   s.per = int((tiles + nseg - 1) / nseg);

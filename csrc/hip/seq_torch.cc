@@ -7,10 +7,12 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <optional>
 
@@ -52,6 +54,20 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+
+// Inside a graph's capture, a leaf whose gradient accumulator an eager graph on the default stream keeps alive would have
+// the captured backward pass wait on that stream, which ends the process. Said here instead.
+void check_capture(std::initializer_list<const Tensor*> leaves) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const Tensor* t : leaves) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (accumulator == nullptr) continue;
+    const auto stream = accumulator->stream();
+    TORCH_CHECK(!stream || stream->id() != 0, "a graph made outside the capture still holds a leaf of this call: "
+                "release its outputs, or capture with leaves of its own");
+  }
 }
 
 // Gradients that say so when they are differentiated again. Only a pass with create_graph runs with gradients enabled.
@@ -114,6 +130,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
 Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, int64_t pad, int64_t type) {
   const Tensor i = ids.contiguous();
   if (!wants_grad({&weight})) return embedding_run(i, weight, scale, type_of(type));
+  check_capture({&weight});
   return Embedding::apply(i, weight, scale, pad, type);
 }
 
@@ -157,6 +174,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 Tensor dropout(const Tensor& x, const OptTensor& res, double p, uint64_t seed, uint64_t offset, const OptTensor& ctr) {
   const Tensor r = plain(res);
   if (!wants_grad({&x, &r})) return dropout_run(x, r, p, int64_t(seed), int64_t(offset), plain(ctr), Tensor());
+  check_capture({&x, &r});
   return Dropout::apply(x, res, p, int64_t(seed), int64_t(offset), ctr);
 }
 
@@ -258,6 +276,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const OptTensor& gate, co
     auto [y, last, ckpt] = scan_run(rows(x), gate ? rows(g) : g, state, plain(r), plain(n), false);
     return {y, last};
   }
+  check_capture({&x, &g, &state});
   const variable_list out = GatedScan::apply(x, gate, h, r, n);
   return {out[0], out[1]};
 }
@@ -271,6 +290,7 @@ std::tuple<Tensor, Tensor> gated_scan_step(const Tensor& x, const OptTensor& gat
   const void* gp = g.defined() ? ptr(g) : static_cast<char*>(ptr(xr)) + D * xr.element_size();
   rmm::hip::gated_scan_step(ptr(xr), xr.stride(0), gp, g.defined() ? g.stride(0) : xr.stride(0), ptr<const uint8_t>(r),
                             ptr<const float>(state), ptr<float>(to), ptr(y), code(x.scalar_type()), B, D, stream_of(x));
+  if (out) torch::autograd::impl::bump_version(to);  // written in place
   return {y, to};
 }
 

@@ -155,6 +155,37 @@ def test_streams_and_threads_at_once():
             assert torch.equal(a, b)
 
 
+def test_a_capture_over_leaves_of_a_living_eager_graph_is_refused():
+    x = torch.randn(2, 6, 4, device="cuda", requires_grad=True)
+    w = torch.randn(5, 4, device="cuda", requires_grad=True)
+    ids = torch.zeros(3, dtype=torch.long, device="cuda")
+    calls = [lambda: ops.dropout(x, 0.5, 1), lambda: ops.gated_scan(x, x.detach())[0], lambda: ops.embedding(ids, w)]
+    alive = [c() for c in calls]
+    for c in calls:
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="outside the capture"):
+            with torch.cuda.graph(graph):
+                c()
+    del alive
+    for c in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = c()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, c())
+        del out
+
+
+def test_a_step_in_place_is_noticed_by_autograd(cuda):
+    state = torch.randn(2, 4, device=cuda)
+    y = torch.ones(2, 4, device=cuda, requires_grad=True) * state
+    with torch.no_grad():
+        ops.gated_scan_step(torch.zeros(2, 4, device=cuda), torch.zeros(2, 4, device=cuda), state, out=state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_second_derivatives_are_refused():
     x = torch.randn(2, 5, 8, device="cuda", requires_grad=True)
     w = torch.randn(6, 8, device="cuda", requires_grad=True)

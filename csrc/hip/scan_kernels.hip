@@ -70,15 +70,19 @@ __device__ __forceinline__ Map then(const Map& first, const Map& later) {
   return Map{first.A == 0.f ? 0.f : fmaxf(first.A * later.A, kTiny), fmaf(later.A, first.H, later.H)};
 }
 
-// Which sequence, channels and segment a workgroup has, and where its wave stands.
+// Which sequence, channels and segment a workgroup has, and where this lane stands. A wave's lanes share a row of
+// 1 << lpr lanes (all 64 unless the tensor is narrow); with fewer, the wave has several groups, each at a chunk of its own.
 struct ScanPlace {
   int64_t b, d;
-  int seg, wave, lane, waves;
+  int seg, wave, lane, waves, lpr, group, groups;
+
+  __device__ int column(int vec) const { return (lane & ((1 << lpr) - 1)) * vec; }
 };
 
-template <int VEC>
-__device__ __forceinline__ ScanPlace scan_place(const ScanArgs& p) {
-  const uint32_t tiles = uint32_t((p.D + kWave * VEC - 1) / (kWave * VEC)), chains = uint32_t(p.B) * tiles;
+template <int VEC, bool NARROW>
+__device__ __forceinline__ ScanPlace scan_place(const ScanArgs& p, int lpr) {
+  if (!NARROW) lpr = 6;
+  const uint32_t tiles = uint32_t((p.D + (VEC << lpr) - 1) / (VEC << lpr)), chains = uint32_t(p.B) * tiles;
   const uint32_t seg = blockIdx.x / chains, chain = blockIdx.x - seg * chains, b = chain / tiles;
   ScanPlace s;
   s.seg = int(seg);
@@ -86,14 +90,25 @@ __device__ __forceinline__ ScanPlace scan_place(const ScanArgs& p) {
   s.lane = threadIdx.x % kWave;
   s.wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   s.waves = blockDim.x / kWave;
-  s.d = (int64_t(chain - b * tiles) * kWave + s.lane) * VEC;
+  s.lpr = lpr;
+  s.group = NARROW ? s.lane >> lpr : 0;
+  s.groups = NARROW ? kWave >> lpr : 1;
+  s.d = (int64_t(chain - b * tiles) << lpr) * VEC + s.column(VEC);
   return s;
 }
 
-// Bits of the first cnt (< 32) steps that have a reset; the same in every lane.
-__device__ __forceinline__ uint32_t reset_bits(const uint8_t* __restrict__ resets, int64_t at, int lane, int cnt) {
+// Bits of the first cnt (<= K < 32) steps from `at` on that have a reset, for each group of lanes.
+template <bool NARROW, int K>
+__device__ __forceinline__ uint32_t reset_bits(const uint8_t* __restrict__ resets, const ScanPlace& s, int64_t at, int cnt) {
   if (resets == nullptr) return 0;
-  return uint32_t(__ballot(lane < cnt && resets[at + lane] != 0));
+  if (!NARROW) return uint32_t(__ballot(s.lane < cnt && resets[at + s.lane] != 0));
+  const int size = 1 << s.lpr, j = s.lane & (size - 1);
+  uint32_t bits = 0;
+  for (int r = 0; r < K; r += size) {
+    const uint64_t m = __ballot(r + j < cnt && resets[at + r + j] != 0);
+    bits |= uint32_t((m >> (s.group << s.lpr)) & ((uint64_t(1) << size) - 1)) << r;
+  }
+  return bits;
 }
 
 template <typename T, int VEC, int K>
@@ -108,15 +123,32 @@ __device__ __forceinline__ void load_rows(const T* __restrict__ p, int64_t strid
   }
 }
 
-// The state that enters this wave's chunk, from the state before the tile (`carry`, which goes on to that behind it) and
-// the compositions of the tile's waves, in the order of the recurrence. `maps` alternates between two buffers from tile to
-// tile, so that one barrier a tile is enough.
+// The groups' maps composed in the order of the recurrence: m becomes that of all groups up to this one.
 template <int VEC>
-__device__ __forceinline__ void exchange(const ScanPlace& s, bool forward, Map (*maps)[kWave * VEC], const Map (&mine)[VEC],
-                                         float (&carry)[VEC], float (&in)[VEC]) {
-  const int at = s.lane * VEC;
+__device__ __forceinline__ void join_groups(const ScanPlace& s, bool forward, Map (&m)[VEC]) {
+  for (int off = 1; off < s.groups; off <<= 1) {
+    const bool has = forward ? s.group >= off : s.group + off < s.groups;
+    const int from = has ? s.lane + (forward ? -off : off) * (1 << s.lpr) : s.lane;
 #pragma unroll
-  for (int v = 0; v < VEC; v++) maps[s.wave][at + v] = mine[v];
+    for (int v = 0; v < VEC; v++) {
+      const Map o{__shfl(m[v].A, from), __shfl(m[v].H, from)};
+      if (has) m[v] = then(o, m[v]);
+    }
+  }
+}
+
+// The state that enters this lane's chunk, from the state before the tile (`carry`, which goes on to that behind it) and
+// the compositions of the tile's chunks, in the order of the recurrence. `maps` alternates between two buffers from tile
+// to tile, so that one barrier a tile is enough.
+template <int VEC, bool NARROW>
+__device__ __forceinline__ void exchange(const ScanPlace& s, bool forward, Map (*maps)[kWave * VEC], Map (&mine)[VEC],
+                                         float (&carry)[VEC], float (&in)[VEC]) {
+  const int at = s.column(VEC);
+  if (NARROW) join_groups<VEC>(s, forward, mine);
+  if (!NARROW || s.group == (forward ? s.groups - 1 : 0)) {
+#pragma unroll
+    for (int v = 0; v < VEC; v++) maps[s.wave][at + v] = mine[v];
+  }
   __syncthreads();
   for (int k = 0; k < s.waves; k++) {
     const int w = forward ? k : s.waves - 1 - k;
@@ -124,6 +156,15 @@ __device__ __forceinline__ void exchange(const ScanPlace& s, bool forward, Map (
     for (int v = 0; v < VEC; v++) {
       if (w == s.wave) in[v] = carry[v];
       carry[v] = apply(maps[w][at + v], carry[v]);
+    }
+  }
+  if (NARROW) {  // through the groups of this wave that come before
+    const bool has = forward ? s.group > 0 : s.group + 1 < s.groups;
+    const int from = has ? s.lane + (forward ? -1 : 1) * (1 << s.lpr) : s.lane;
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+      const Map o{__shfl(mine[v].A, from), __shfl(mine[v].H, from)};
+      if (has) in[v] = apply(o, in[v]);
     }
   }
 }
@@ -152,7 +193,7 @@ struct Chunk {
   uint32_t resets;
 };
 
-template <int K>
+template <bool NARROW, int K>
 __device__ __forceinline__ Chunk chunk_of(const ScanArgs& p, const ScanPlace& s, int n, int ck) {
   Chunk c;
   c.ck = ck;
@@ -160,8 +201,15 @@ __device__ __forceinline__ Chunk chunk_of(const ScanArgs& p, const ScanPlace& s,
   c.t0 = t0;
   c.rows = max(0, min(K, L - t0));
   c.cnt = max(0, min(K, n - t0));
-  c.resets = reset_bits(p.resets, s.b * p.L + t0, s.lane, c.cnt);
+  c.resets = reset_bits<NARROW, K>(p.resets, s, s.b * p.L + t0, c.cnt);
   return c;
+}
+
+// Whether the chunk's steps all take part, without a reset, in every lane.
+template <bool NARROW, int K>
+__device__ __forceinline__ bool is_plain(const Chunk& c) {
+  const bool plain = c.cnt == K && c.resets == 0;
+  return NARROW ? __all(plain) : plain;
 }
 
 // The chunk's factor of the state before it, from the plain product of its steps' factors.
@@ -212,19 +260,20 @@ __device__ __forceinline__ void write_states(const Chunk& c, const float (&aa)[K
 }
 
 // `per` tiles in a segment.
-template <typename T, int VEC>
-__global__ __launch_bounds__(kScanThreads, 4) void k_scan_fwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
-                                                           T* __restrict__ y, int nseg, int per,
-                                                           const Map* __restrict__ seg_maps) {
+template <typename T, int VEC, bool NARROW>
+__global__ __launch_bounds__(kScanThreads, NARROW ? 2 : 4) void k_scan_fwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
+                                                              T* __restrict__ y, int nseg, int per, int lpr,
+                                                              const Map* __restrict__ seg_maps) {
   constexpr int K = chunk_steps<T>();
   __shared__ Map maps[2][kScanWaves][kWave * VEC];
-  const ScanPlace s = scan_place<VEC>(p);
+  const ScanPlace s = scan_place<VEC, NARROW>(p, lpr);
   const bool live = s.d < p.D;
-  const int n = length_of(p.lengths, s.b, int(p.L)), nck = int((p.L + K - 1) / K);
-  const int first = s.seg * per, last = max(first + 1, min(first + per, (nck + s.waves - 1) / s.waves));
+  const int n = length_of(p.lengths, s.b, int(p.L)), nck = int((p.L + K - 1) / K), units = s.waves * s.groups;
+  const int unit = s.wave * s.groups + s.group;
+  const int first = s.seg * per, last = max(first + 1, min(first + per, (nck + units - 1) / units));
   const T *xp = x + s.b * p.xsb + s.d, *gp = g + s.b * p.gsb + s.d;
   VecOf<T, VEC> xr[K], gr[K];
-  Chunk c = chunk_of<K>(p, s, n, first * s.waves + s.wave);
+  Chunk c = chunk_of<NARROW, K>(p, s, n, first * units + unit);
   if (live) {
     load_rows<T, VEC, K>(gp + c.t0 * p.gst, p.gst, c.cnt, gr);
     load_rows<T, VEC, K>(xp + c.t0 * p.xst, p.xst, c.cnt, xr);
@@ -235,19 +284,19 @@ __global__ __launch_bounds__(kScanThreads, 4) void k_scan_fwd(ScanArgs p, const 
     float aa[K][VEC], uu[K][VEC], in[VEC];
     Map m[VEC];
     const Chunk now = c;
-    const bool plain = now.cnt == K && now.resets == 0;
+    const bool plain = is_plain<NARROW, K>(now);
     if (plain)
       compose<true, T, VEC, K>(now, xr, gr, aa, uu, m);
     else
       compose<false, T, VEC, K>(now, xr, gr, aa, uu, m);
     if (tile + 1 < last) {
-      c = chunk_of<K>(p, s, n, (tile + 1) * s.waves + s.wave);
+      c = chunk_of<NARROW, K>(p, s, n, (tile + 1) * units + unit);
       if (live) {
         load_rows<T, VEC, K>(gp + c.t0 * p.gst, p.gst, c.cnt, gr);
         load_rows<T, VEC, K>(xp + c.t0 * p.xst, p.xst, c.cnt, xr);
       }
     }
-    exchange<VEC>(s, true, maps[tile & 1], m, carry, in);
+    exchange<VEC, NARROW>(s, true, maps[tile & 1], m, carry, in);
     if (!live) continue;
     if (now.rows > 0 && p.ckpt) store_vec<float, VEC>(p.ckpt + (s.b * nck + now.ck) * p.D + s.d, in);
     T* yp = y + (s.b * p.L + now.t0) * p.D + s.d;
@@ -256,7 +305,7 @@ __global__ __launch_bounds__(kScanThreads, 4) void k_scan_fwd(ScanArgs p, const 
     else
       write_states<false, T, VEC, K>(now, aa, uu, in, yp, p.D);
   }
-  if (live && s.wave == 0 && s.seg == nseg - 1) store_vec<float, VEC>(p.h_last + s.b * p.D + s.d, carry);
+  if (live && unit == 0 && s.seg == nseg - 1) store_vec<float, VEC>(p.h_last + s.b * p.D + s.d, carry);
 }
 
 // One chunk backward: z, 1 - z and the gate's factor dg / dh (cc) of each step, and the chunk's map of the state's
@@ -320,23 +369,24 @@ __device__ __forceinline__ void write_grads(const Chunk& c, const VecOf<T, VEC> 
   }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool NARROW>
 __global__ __launch_bounds__(kScanThreads) void k_scan_bwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
                                                            const T* __restrict__ dy, T* __restrict__ dx,
-                                                           T* __restrict__ dg, int nseg, int per,
+                                                           T* __restrict__ dg, int nseg, int per, int lpr,
                                                            const Map* __restrict__ seg_maps) {
   constexpr int K = chunk_steps<T>();
   __shared__ Map maps[2][kScanWaves][kWave * VEC];
-  const ScanPlace s = scan_place<VEC>(p);  // segment 0 is the last in time, where this pass begins
+  const ScanPlace s = scan_place<VEC, NARROW>(p, lpr);  // segment 0 is the last in time, where this pass begins
   const bool live = s.d < p.D;
-  const int n = length_of(p.lengths, s.b, int(p.L)), nck = int((p.L + K - 1) / K);
-  const int first = (nseg - 1 - s.seg) * per, last = max(first + 1, min(first + per, (nck + s.waves - 1) / s.waves));
+  const int n = length_of(p.lengths, s.b, int(p.L)), nck = int((p.L + K - 1) / K), units = s.waves * s.groups;
+  const int unit = s.wave * s.groups + s.group;
+  const int first = (nseg - 1 - s.seg) * per, last = max(first + 1, min(first + per, (nck + units - 1) / units));
   const T *xp = x + s.b * p.xsb + s.d, *gp = g + s.b * p.gsb + s.d, *yp = dy ? dy + s.b * p.ysb + s.d : nullptr;
   VecOf<T, VEC> xr[K], gr[K], yr[K];
   float h[VEC] = {};
   Chunk c;
   const auto load = [&](int tile) {
-    c = chunk_of<K>(p, s, n, tile * s.waves + s.wave);
+    c = chunk_of<NARROW, K>(p, s, n, tile * units + unit);
     if (!live) return;
     if (c.cnt > 0) load_vec<float, VEC>(p.ckpt + (s.b * nck + c.ck) * p.D + s.d, h);
     load_rows<T, VEC, K>(gp + c.t0 * p.gst, p.gst, c.cnt, gr);
@@ -351,7 +401,7 @@ __global__ __launch_bounds__(kScanThreads) void k_scan_bwd(ScanArgs p, const T* 
     VecOf<T, VEC> yn[K];
     Map m[VEC];
     const Chunk now = c;
-    const bool plain = now.cnt == K && now.resets == 0 && dy != nullptr;
+    const bool plain = is_plain<NARROW, K>(now) && dy != nullptr;
     if (plain)
       compose_back<true, T, VEC, K>(now, xr, gr, yr, true, h, zz, aa, cc, m);
     else
@@ -359,7 +409,7 @@ __global__ __launch_bounds__(kScanThreads) void k_scan_bwd(ScanArgs p, const T* 
 #pragma unroll
     for (int i = 0; i < K; i++) yn[i] = yr[i];
     if (tile > first) load(tile - 1);
-    exchange<VEC>(s, false, maps[tile & 1], m, carry, in);
+    exchange<VEC, NARROW>(s, false, maps[tile & 1], m, carry, in);
     if (!live) continue;
     T *dxp = dx + s.b * p.dsb + now.t0 * p.dst + s.d, *dgp = dg + s.b * p.dsb + now.t0 * p.dst + s.d;
     if (plain)
@@ -367,7 +417,7 @@ __global__ __launch_bounds__(kScanThreads) void k_scan_bwd(ScanArgs p, const T* 
     else
       write_grads<false, T, VEC, K>(now, yn, dy != nullptr, zz, aa, cc, in, dxp, dgp, p.dst);
   }
-  if (live && p.dh0 && s.wave == 0 && s.seg == nseg - 1) store_vec<float, VEC>(p.dh0 + s.b * p.D + s.d, carry);
+  if (live && p.dh0 && unit == 0 && s.seg == nseg - 1) store_vec<float, VEC>(p.dh0 + s.b * p.D + s.d, carry);
 }
 
 // m becomes the chunk's map: forward of (gate, input), backward of (gate, dy).
@@ -403,24 +453,26 @@ __device__ __forceinline__ void compose_map(const Chunk& c, const VecOf<T, VEC> 
 // in a segment. Little is kept from chunk to chunk, so 32 waves a CU hide the loads.
 constexpr int kMapWaves = 16;
 
-template <typename T, int VEC, bool FORWARD>
-__global__ __launch_bounds__(kMapWaves* kWave, 8) void k_scan_maps(ScanArgs p, const T* __restrict__ g,
+template <typename T, int VEC, bool NARROW, bool FORWARD>
+__global__ __launch_bounds__(kMapWaves* kWave, NARROW || sizeof(T) == 4 ? 4 : 8) void k_scan_maps(ScanArgs p, const T* __restrict__ g,
                                                                    const T* __restrict__ in, int nseg, int len,
-                                                                   Map* __restrict__ seg_maps) {
+                                                                   int lpr, Map* __restrict__ seg_maps) {
   constexpr int K = chunk_steps<T>();
   __shared__ Map maps[kMapWaves][kWave * VEC];
-  const ScanPlace s = scan_place<VEC>(p);
+  const ScanPlace s = scan_place<VEC, NARROW>(p, lpr);
   const bool live = s.d < p.D;
-  const int n = length_of(p.lengths, s.b, int(p.L)), nck = int((p.L + K - 1) / K);
+  const int n = length_of(p.lengths, s.b, int(p.L)), nck = int((p.L + K - 1) / K), units = s.waves * s.groups;
   const int begin = (FORWARD ? s.seg : nseg - 1 - s.seg) * len, end = min(begin + len, nck);
-  const int each = (len + s.waves - 1) / s.waves, lo = min(begin + s.wave * each, end), hi = min(lo + each, end);
+  const int each = (len + units - 1) / units, lo = min(begin + (s.wave * s.groups + s.group) * each, end);
+  const int hi = min(lo + each, end);
   const int64_t isb = FORWARD ? p.xsb : p.ysb, ist = FORWARD ? p.xst : p.yst;
   const T *gp = g + s.b * p.gsb + s.d, *ip = in ? in + s.b * isb + s.d : nullptr;
   Map m[VEC];
 #pragma unroll
   for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
-  for (int k = 0; k < hi - lo; k++) {
-    const Chunk c = chunk_of<K>(p, s, n, FORWARD ? lo + k : hi - 1 - k);
+  for (int k = 0; k < (NARROW ? each : hi - lo); k++) {  // the same count for all lanes of a wave
+    const int ck = FORWARD ? lo + k : hi - 1 - k;
+    const Chunk c = chunk_of<NARROW, K>(p, s, NARROW && k >= hi - lo ? 0 : n, ck);
     if (!live || c.cnt == 0) continue;
     VecOf<T, VEC> gr[K], ir[K];
     load_rows<T, VEC, K>(gp + c.t0 * p.gst, p.gst, c.cnt, gr);
@@ -433,14 +485,18 @@ __global__ __launch_bounds__(kMapWaves* kWave, 8) void k_scan_maps(ScanArgs p, c
 #pragma unroll
     for (int v = 0; v < VEC; v++) m[v] = then(m[v], cm[v]);
   }
+  if (NARROW) join_groups<VEC>(s, FORWARD, m);
+  const int at = s.column(VEC);
+  if (!NARROW || s.group == (FORWARD ? s.groups - 1 : 0)) {
 #pragma unroll
-  for (int v = 0; v < VEC; v++) maps[s.wave][s.lane * VEC + v] = m[v];
+    for (int v = 0; v < VEC; v++) maps[s.wave][at + v] = m[v];
+  }
   __syncthreads();
-  if (s.wave != 0 || !live) return;
+  if (s.wave != 0 || s.group != 0 || !live) return;
 #pragma unroll
   for (int v = 0; v < VEC; v++) {
     Map all{1.f, 0.f};
-    for (int k = 0; k < s.waves; k++) all = then(all, maps[FORWARD ? k : s.waves - 1 - k][s.lane * VEC + v]);
+    for (int k = 0; k < s.waves; k++) all = then(all, maps[FORWARD ? k : s.waves - 1 - k][at + v]);
     seg_maps[(s.seg * p.B + s.b) * p.D + s.d + v] = all;
   }
 }
@@ -461,7 +517,7 @@ __global__ __launch_bounds__(256) void k_scan_step(const T* __restrict__ x, int6
 }
 
 struct ScanPlan {
-  int waves = 1, per = 1, nseg = 1;
+  int waves = 1, per = 1, nseg = 1, lpr = 6, units = 1;
   int64_t chains = 0;
 };
 
@@ -474,11 +530,14 @@ int steps_of(int type) { return type == kF32 ? chunk_steps<float>() : chunk_step
 constexpr int64_t kEnoughChains = 128, kGroups = 256;
 
 ScanPlan scan_plan(const ScanArgs& p, int type, int vec, const char* who) {
-  if (p.L >= (int64_t(1) << 31) - 4096) throw std::invalid_argument(std::string(who) + ": too many steps");
+  if (p.L >= (int64_t(1) << 31) - 65536) throw std::invalid_argument(std::string(who) + ": too many steps");
   ScanPlan s;
   const int64_t chunks = std::max<int64_t>(1, (p.L + steps_of(type) - 1) / steps_of(type));
-  s.waves = int(std::min<int64_t>(kScanWaves, chunks));
-  const int64_t tiles = (chunks + s.waves - 1) / s.waves, cols = (p.D + kWave * vec - 1) / (kWave * vec);
+  while (s.lpr > 0 && p.D <= (vec << (s.lpr - 1))) s.lpr--;
+  const int groups = kWave >> s.lpr;
+  s.waves = int(std::min<int64_t>(kScanWaves, (chunks + groups - 1) / groups));
+  s.units = s.waves * groups;
+  const int64_t tiles = (chunks + s.units - 1) / s.units, cols = (p.D + (vec << s.lpr) - 1) / (vec << s.lpr);
   if (p.B > ((int64_t(1) << 31) - 1) / cols) throw std::invalid_argument(std::string(who) + ": too many sequences");
   s.chains = p.B * cols;
   int64_t nseg = s.chains >= kEnoughChains ? 1 : std::min(tiles, kGroups / s.chains);
@@ -496,33 +555,29 @@ bool pairs(const ScanArgs& p, std::initializer_list<const void*> ptrs) {
   return true;
 }
 
-template <typename T, int VEC>
-void scan_fwd_t(const ScanArgs& p, const T* x, const T* g, T* y, int type, hipStream_t stream) {
-  const ScanPlan s = scan_plan(p, type, VEC, "gated_scan");
-  Map* maps = static_cast<Map*>(p.workspace);
-  const dim3 block(uint32_t(s.waves * kWave));
-  if (s.nseg > 1) {
-    if (maps == nullptr) throw std::invalid_argument("gated_scan: no workspace");
-    hipLaunchKernelGGL((k_scan_maps<T, VEC, true>), dim3(uint32_t(s.chains * (s.nseg - 1))), dim3(kMapWaves * kWave), 0,
-                       stream, p, g, x, s.nseg, s.per * s.waves, maps);
-  }
-  hipLaunchKernelGGL((k_scan_fwd<T, VEC>), dim3(uint32_t(s.chains * s.nseg)), block, 0, stream, p, x, g, y, s.nseg, s.per,
-                     maps);
+template <typename T, int VEC, bool NARROW, bool FORWARD>
+void scan_maps_t(const ScanArgs& p, const ScanPlan& s, const T* g, const T* in, const char* who, hipStream_t stream) {
+  if (s.nseg == 1) return;
+  if (p.workspace == nullptr) throw std::invalid_argument(std::string(who) + ": no workspace");
+  hipLaunchKernelGGL((k_scan_maps<T, VEC, NARROW, FORWARD>), dim3(uint32_t(s.chains * (s.nseg - 1))),
+                     dim3(kMapWaves * kWave), 0, stream, p, g, in, s.nseg, s.per * s.units, s.lpr,
+                     static_cast<Map*>(p.workspace));
+}
+
+template <typename T, int VEC, bool NARROW>
+void scan_fwd_t(const ScanArgs& p, const ScanPlan& s, const T* x, const T* g, T* y, hipStream_t stream) {
+  scan_maps_t<T, VEC, NARROW, true>(p, s, g, x, "gated_scan", stream);
+  hipLaunchKernelGGL((k_scan_fwd<T, VEC, NARROW>), dim3(uint32_t(s.chains * s.nseg)), dim3(uint32_t(s.waves * kWave)), 0,
+                     stream, p, x, g, y, s.nseg, s.per, s.lpr, static_cast<const Map*>(p.workspace));
   RMM_HIP_CHECK(hipGetLastError());
 }
 
-template <typename T, int VEC>
-void scan_bwd_t(const ScanArgs& p, const T* x, const T* g, const T* dy, T* dx, T* dg, int type, hipStream_t stream) {
-  const ScanPlan s = scan_plan(p, type, VEC, "gated_scan backward");
-  Map* maps = static_cast<Map*>(p.workspace);
-  const dim3 block(uint32_t(s.waves * kWave));
-  if (s.nseg > 1) {
-    if (maps == nullptr) throw std::invalid_argument("gated_scan backward: no workspace");
-    hipLaunchKernelGGL((k_scan_maps<T, VEC, false>), dim3(uint32_t(s.chains * (s.nseg - 1))), dim3(kMapWaves * kWave), 0,
-                       stream, p, g, dy, s.nseg, s.per * s.waves, maps);
-  }
-  hipLaunchKernelGGL((k_scan_bwd<T, VEC>), dim3(uint32_t(s.chains * s.nseg)), block, 0, stream, p, x, g, dy, dx, dg, s.nseg,
-                     s.per, maps);
+template <typename T, int VEC, bool NARROW>
+void scan_bwd_t(const ScanArgs& p, const ScanPlan& s, const T* x, const T* g, const T* dy, T* dx, T* dg,
+                hipStream_t stream) {
+  scan_maps_t<T, VEC, NARROW, false>(p, s, g, dy, "gated_scan backward", stream);
+  hipLaunchKernelGGL((k_scan_bwd<T, VEC, NARROW>), dim3(uint32_t(s.chains * s.nseg)), dim3(uint32_t(s.waves * kWave)), 0,
+                     stream, p, x, g, dy, dx, dg, s.nseg, s.per, s.lpr, static_cast<const Map*>(p.workspace));
   RMM_HIP_CHECK(hipGetLastError());
 }
 
@@ -542,8 +597,11 @@ void gated_scan_fwd(const ScanArgs& p, const void* x, const void* g, void* y, in
   if (p.B <= 0 || p.D <= 0) return;
   dispatch_type(type, "gated_scan", [&](auto tag) {
     using T = decltype(tag);
-    const auto fwd = pairs<T>(p, {x, g, y}) ? scan_fwd_t<T, 2> : scan_fwd_t<T, 1>;
-    fwd(p, static_cast<const T*>(x), static_cast<const T*>(g), static_cast<T*>(y), type, stream);
+    const int vec = pairs<T>(p, {x, g, y}) ? 2 : 1;
+    const ScanPlan s = scan_plan(p, type, vec, "gated_scan");
+    const auto fwd = vec == 2 ? (s.lpr < 6 ? scan_fwd_t<T, 2, true> : scan_fwd_t<T, 2, false>)
+                              : (s.lpr < 6 ? scan_fwd_t<T, 1, true> : scan_fwd_t<T, 1, false>);
+    fwd(p, s, static_cast<const T*>(x), static_cast<const T*>(g), static_cast<T*>(y), stream);
   });
 }
 
@@ -553,9 +611,12 @@ void gated_scan_bwd(const ScanArgs& p, const void* x, const void* g, const void*
   if (p.L > 0 && p.ckpt == nullptr) throw std::invalid_argument("gated_scan backward: no saved states");
   dispatch_type(type, "gated_scan backward", [&](auto tag) {
     using T = decltype(tag);
-    const auto bwd = pairs<T>(p, {x, g, dy, dx, dg}) ? scan_bwd_t<T, 2> : scan_bwd_t<T, 1>;
-    bwd(p, static_cast<const T*>(x), static_cast<const T*>(g), static_cast<const T*>(dy), static_cast<T*>(dx),
-        static_cast<T*>(dg), type, stream);
+    const int vec = pairs<T>(p, {x, g, dy, dx, dg}) ? 2 : 1;
+    const ScanPlan s = scan_plan(p, type, vec, "gated_scan backward");
+    const auto bwd = vec == 2 ? (s.lpr < 6 ? scan_bwd_t<T, 2, true> : scan_bwd_t<T, 2, false>)
+                              : (s.lpr < 6 ? scan_bwd_t<T, 1, true> : scan_bwd_t<T, 1, false>);
+    bwd(p, s, static_cast<const T*>(x), static_cast<const T*>(g), static_cast<const T*>(dy), static_cast<T*>(dx),
+        static_cast<T*>(dg), stream);
   });
 }
 

@@ -29,28 +29,32 @@ __device__ __forceinline__ uint32_t embed_key(TI id, int64_t V, int64_t pad) {
 }
 
 // ------------------------------------------------------------------------------------------ lookup
-// 2^lpr lanes share a row (VEC elements each); a workgroup has 256 >> lpr rows in flight.
+// 2^lpr lanes share a row (VEC elements each, up to kRun times); a workgroup has 256 >> lpr rows in flight.
+constexpr int kRun = 4;
+
 template <typename TI, typename TW, typename TO, int VEC>
 __global__ __launch_bounds__(256) void k_embed_fwd(const TI* __restrict__ ids, const TW* __restrict__ w, int64_t ws,
                                                    TO* __restrict__ out, int64_t n, int64_t V, int64_t D, float scale,
                                                    int lpr) {
   const int lane = threadIdx.x & ((1 << lpr) - 1);
-  const int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) >> lpr;
+  const int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) >> lpr, step = int64_t(VEC) << lpr;
   if (i >= n) return;
   const int64_t id = int64_t(ids[i]);
   const bool ok = id >= 0 && id < V;
   const TW* row = w + (ok ? id : 0) * ws;
-  for (int64_t c = int64_t(lane) * VEC; c < D; c += int64_t(VEC) << lpr) {
-    float v[VEC];
-    if (ok) {
-      load_vec<TW, VEC>(row + c, v);
+  for (int64_t c0 = int64_t(lane) * VEC; c0 < D; c0 += kRun * step) {
+    VecOf<TW, VEC> r[kRun];
 #pragma unroll
-      for (int k = 0; k < VEC; k++) v[k] *= scale;
-    } else {
+    for (int q = 0; q < kRun; q++)
+      if (ok && c0 + q * step < D) r[q] = *reinterpret_cast<const VecOf<TW, VEC>*>(row + c0 + q * step);
 #pragma unroll
-      for (int k = 0; k < VEC; k++) v[k] = 0.f;
+    for (int q = 0; q < kRun; q++) {
+      if (c0 + q * step >= D) break;
+      float v[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; k++) v[k] = ok ? to_f32(r[q].v[k]) * scale : 0.f;
+      store_vec<TO, VEC>(out + i * D + c0 + q * step, v);
     }
-    store_vec<TO, VEC>(out + i * D + c, v);
   }
 }
 
@@ -465,7 +469,8 @@ void embed_fwd_t(const TI* ids, const void* w, int64_t ws, void* out, int64_t n,
   const auto run = [&](auto width) {
     constexpr int VEC = decltype(width)::value;
     if (D % VEC || ws % VEC || !vec_aligned<TW, VEC>(w) || !vec_aligned<TO, VEC>(out)) return false;
-    const int lpr = lanes_log2(D, VEC);
+    // a wave a row where there are rows enough to fill the card, else up to a workgroup a row
+    const int lpr = std::min(lanes_log2(D, VEC), n >= 4096 ? 6 : 8);
     hipLaunchKernelGGL((k_embed_fwd<TI, TW, TO, VEC>), dim3(row_blocks(n, lpr, "embedding")), dim3(256), 0, stream, ids,
                        wp, ws, op, n, V, D, scale, lpr);
     RMM_HIP_CHECK(hipGetLastError());

@@ -4,7 +4,8 @@ autograd in ``csrc/hip/seq_torch.cc``).
 
 CUDA(ROCm) tensors run the HIP kernels on the current stream of their device; CPU tensors the same formulas in torch.
 fp32, bf16 and fp16 are taken on the GPU; sums and states are held in fp32. Everything here can be captured into a
-graph: nothing synchronises, and what a call keeps for its backward pass belongs to that call.
+graph: nothing synchronises, and what a call keeps for its backward pass belongs to that call. (A capture refuses leaves
+that a graph made outside it still holds: torch's engine would have the captured backward pass wait on their stream.)
 """
 from __future__ import annotations
 
@@ -83,8 +84,8 @@ class Embedding(nn.Embedding):
     """``nn.Embedding`` through :func:`embedding`: the same parameters and state dict, with a ``scale`` on the output.
     ``max_norm``, ``scale_grad_by_freq`` and ``sparse`` are not supported."""
 
-    def __init__(self, num_embeddings: int, embedding_dim: int, padding_idx: Optional[int] = None, scale: float = 1.0,
-                 **kw):
+    def __init__(self, num_embeddings: int, embedding_dim: int, padding_idx: Optional[int] = None, *,
+                 scale: float = 1.0, **kw):
         for k in ("max_norm", "scale_grad_by_freq", "sparse"):
             if kw.get(k):
                 raise ValueError(f"Embedding: {k} is not supported")

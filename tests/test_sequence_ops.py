@@ -183,6 +183,7 @@ def test_embedding_module_matches_torch(dev):
     m(ids).sum().backward()
     r(ids).sum().backward()
     assert torch.equal(m.weight.grad, r.weight.grad)  # sums of ones: exact in any order
+    assert torch.equal(ops.Embedding.from_pretrained(r.weight.detach()).to(dev)(ids), r(ids))
     for bad in ({"sparse": True}, {"max_norm": 1.0}, {"scale_grad_by_freq": True}):
         with pytest.raises(ValueError, match="not supported"):
             ops.Embedding(3, 4, **bad)

@@ -7,8 +7,8 @@
 // depend on scheduling: the positions are sorted by id with a stable radix sort (no floating-point
 // atomics) and each row of dW is a walk over its segment of the sorted positions.
 //
-// All of it is bound by memory. 131071 tokens, 1536 columns, fp32 table of 100003 rows under bf16 rows: lookup 136 us
-// (402 MB written, 805 MB of rows read of which the caches serve the frequent ones), gradient 290 us = sort 30 + sums 235
+// All of it is bound by memory. 131071 tokens, 1536 columns, fp32 table of 100003 rows under bf16 rows: lookup 143 us
+// (402 MB written, 805 MB of rows read of which the caches serve the frequent ones), gradient 278 us = sort 30 + sums 238
 // (402 MB read, 614 MB written, 4.3 TB/s) + joins 10. 8192 tokens of 1024 bf16 columns, 32768 rows: lookup 7 us, gradient
 // 36 us = sort 18 (one workgroup: its latency) + sums 14 (5.9 TB/s) + joins 4.
 #include <hip/hip_fp16.h>

@@ -572,7 +572,8 @@ void embedding_fwd(const void* ids, bool ids64, const void* w, int wtype, int64_
 
 int64_t embedding_grad_workspace(int64_t n, int64_t V, int64_t D) {
   if (n <= 0 || D <= 0) return 0;
-  const int64_t pieces = (n + 15) / 16;  // the shortest
+  int64_t pieces = 0;  // of whichever width the launch will have
+  for (int vec : {8, 4, 2, 1}) pieces = std::max(pieces, sum_plan(n, D, vec, vec >= 4).pieces);
   return (sort_words(n, V) + 3) / 4 * 16 + (pieces > 1 ? 2 * pieces * D * int64_t(sizeof(float)) : 0);
 }
 

@@ -252,3 +252,69 @@ def test_a_batch_of_many_short_sequences(cuda):
     y, h = ops.gated_scan(x, torch.zeros_like(x))
     want = x[:, 0] / 2
     assert torch.equal(y[:, 0], want) and torch.allclose(y[:, 1], want / 2 + x[:, 1] / 2) and torch.equal(h, y[:, 1])
+
+
+def batch_reference(x, g, h0, resets, lengths, dy, dh):
+    """test_sequence_ops.scan_reference (values and bounds) for all sequences at once."""
+    u = 2.0 ** -24
+    x, g, dy = x.double(), g.double(), dy.double()
+    B, L, D = x.shape
+    live = (torch.arange(L, device=x.device)[None] < lengths[:, None])[:, :, None]
+    z, a = torch.sigmoid(g), torch.sigmoid(-g)
+    k = (2 * (g.abs() + 8) + 4) * u
+    cut = resets[:, :, None]
+    h, H = h0.double(), h0.double().abs()
+    E = torch.zeros_like(h)
+    out = {n: torch.zeros(B, L, D, dtype=torch.float64, device=x.device) for n in ("y", "ey", "dx", "ex", "dg", "eg")}
+    hp, Hp, Ep = (torch.zeros_like(out["y"]) for _ in range(3))
+    for t in range(L):
+        keep = (~cut[:, t]).double()
+        hp[:, t], Hp[:, t], Ep[:, t] = h * keep, H * keep, E * keep
+        nh = a[:, t] * hp[:, t] + z[:, t] * x[:, t]
+        nH = a[:, t] * Hp[:, t] + z[:, t] * x[:, t].abs()
+        nE = a[:, t] * Ep[:, t] + k[:, t] * nH
+        h, H, E = (torch.where(live[:, t], n, o) for n, o in ((nh, h), (nH, H), (nE, E)))
+        out["y"][:, t], out["ey"][:, t] = nh, nE
+    out["h"], out["eh"] = h, E
+    back, M = dh.double(), dh.double().abs()
+    F = torch.zeros_like(back)
+    for t in range(L - 1, -1, -1):
+        b, m = back + dy[:, t], M + dy[:, t].abs()
+        f = F + k[:, t] * m
+        diff = x[:, t].abs() + Hp[:, t]
+        out["dx"][:, t], out["ex"][:, t] = b * z[:, t], z[:, t] * (f + k[:, t] * m)
+        out["dg"][:, t] = b * (x[:, t] - hp[:, t]) * z[:, t] * a[:, t]
+        out["eg"][:, t] = z[:, t] * a[:, t] * (f * diff + m * Ep[:, t] + 2 * k[:, t] * m * diff)
+        keep = (~cut[:, t]).double() * a[:, t]
+        back, M, F = (torch.where(live[:, t], n, o) for n, o in (
+            (b * keep, back), (m * keep, M), (f * keep + k[:, t] * m * keep, F)))
+    out["dh0"], out["eh0"] = back, F
+    for n in ("y", "ey", "dx", "ex", "dg", "eg"):
+        out[n] = torch.where(live, out[n], 0.0)
+    return out
+
+
+@pytest.mark.parametrize("B,L,D,t", [
+    (130, 2600, 6, torch.bfloat16), (140, 700, 130, torch.float32), (3, 9000, 20, torch.float16), (128, 400, 64, torch.bfloat16),
+    (2, 5000, 34, torch.float32), (40, 600, 1, torch.bfloat16), (1, 12345, 7, torch.float32), (70, 900, 257, torch.float16)])
+def test_gated_scan_over_many_tiles_and_segments(cuda, B, L, D, t):
+    """Whole and cut chains, wide and narrow rows, odd widths, with resets and lengths."""
+    from test_sequence_ops import check
+
+    g = torch.Generator(device="cuda").manual_seed(B * L + D)
+    x = torch.randn(B, L, D, generator=g, device=cuda).to(t)
+    gate = (torch.randn(B, L, D, generator=g, device=cuda) * 1.5 - 2).to(t)
+    resets = torch.rand(B, L, generator=g, device=cuda) < 0.005
+    lengths = torch.randint(0, L + 1, (B,), generator=g, device=cuda)
+    lengths[0] = L
+    h0, dh = (torch.randn(B, D, generator=g, device=cuda) for _ in range(2))
+    dy = torch.randn(B, L, D, generator=g, device=cuda).to(t)
+    ref = {n: v.cpu() for n, v in batch_reference(x, gate, h0, resets, lengths, dy, dh).items()}
+    leaves = [v.clone().requires_grad_() for v in (x, gate, h0)]
+    y, h = ops.gated_scan(*leaves, resets=resets, lengths=lengths)
+    check(y, ref["y"], ref["ey"], t)
+    check(h, ref["h"], ref["eh"], torch.float32)
+    gx, gg, gh = torch.autograd.grad((y, h), leaves, (dy, dh))
+    check(gx, ref["dx"], ref["ex"], t)
+    check(gg, ref["dg"], ref["eg"], t)
+    check(gh, ref["dh0"], ref["eh0"], torch.float32)

@@ -99,7 +99,9 @@ __device__ __forceinline__ ScanPlace scan_place(const ScanArgs& p, int lpr) {
   s.lpr = lpr;
   s.group = NARROW ? s.lane >> lpr : 0;
   s.groups = NARROW ? kWave >> lpr : 1;
+  // The last pair of an odd row begins one channel earlier: two lanes have that channel and write the same values.
   s.d = (int64_t(chain - b * tiles) << lpr) * VEC + s.column(VEC);
+  if (VEC == 2 && s.d == p.D - 1) s.d--;
   return s;
 }
 
@@ -118,14 +120,14 @@ __device__ __forceinline__ uint32_t reset_bits(const uint8_t* __restrict__ reset
 }
 
 template <typename T, int VEC, int K>
-__device__ __forceinline__ void load_rows(const T* __restrict__ p, int64_t stride, int cnt, VecOf<T, VEC> (&r)[K]) {
+__device__ __forceinline__ void load_rows(const T* __restrict__ p, int64_t stride, int cnt, RunOf<T, VEC> (&r)[K]) {
   if (cnt == K) {
 #pragma unroll
-    for (int i = 0; i < K; i++) r[i] = *reinterpret_cast<const VecOf<T, VEC>*>(p + i * stride);
+    for (int i = 0; i < K; i++) r[i] = *reinterpret_cast<const RunOf<T, VEC>*>(p + i * stride);
   } else {
 #pragma unroll
     for (int i = 0; i < K; i++)
-      if (i < cnt) r[i] = *reinterpret_cast<const VecOf<T, VEC>*>(p + i * stride);
+      if (i < cnt) r[i] = *reinterpret_cast<const RunOf<T, VEC>*>(p + i * stride);
   }
 }
 
@@ -225,7 +227,7 @@ __device__ __forceinline__ float chunk_factor(const Chunk& c, float product) {
 
 // One chunk forward: 1 - z and z x of each step, and the chunk's map. PLAIN: all K steps and no reset.
 template <bool PLAIN, typename T, int VEC, int K>
-__device__ __forceinline__ void compose(const Chunk& c, const VecOf<T, VEC> (&x)[K], const VecOf<T, VEC> (&g)[K],
+__device__ __forceinline__ void compose(const Chunk& c, const RunOf<T, VEC> (&x)[K], const RunOf<T, VEC> (&g)[K],
                                         float (&aa)[K][VEC], float (&uu)[K][VEC], Map (&m)[VEC]) {
 #pragma unroll
   for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
@@ -260,7 +262,7 @@ __device__ __forceinline__ void write_states(const Chunk& c, const float (&aa)[K
         if (has) h[v] = drop ? uu[i][v] : fmaf(aa[i][v], h[v], uu[i][v]);
         o[v] = has ? h[v] : 0.f;
       }
-      store_vec<T, VEC>(y + i * stride, o);
+      store_run<T, VEC>(y + i * stride, o);
     }
   }
 }
@@ -278,7 +280,7 @@ __global__ __launch_bounds__(kScanThreads, NARROW ? 2 : 4) void k_scan_fwd(ScanA
   const int unit = s.wave * s.groups + s.group;
   const int first = s.seg * per, last = max(first + 1, min(first + per, (nck + units - 1) / units));
   const T *xp = x + s.b * p.xsb + s.d, *gp = g + s.b * p.gsb + s.d;
-  VecOf<T, VEC> xr[K], gr[K];
+  RunOf<T, VEC> xr[K], gr[K];
   Chunk c = chunk_of<NARROW, K>(p, s, n, first * units + unit);
   if (live) {
     load_rows<T, VEC, K>(gp + c.t0 * p.gst, p.gst, c.cnt, gr);
@@ -304,21 +306,21 @@ __global__ __launch_bounds__(kScanThreads, NARROW ? 2 : 4) void k_scan_fwd(ScanA
     }
     exchange<VEC, NARROW>(s, true, maps[tile & 1], m, carry, in);
     if (!live) continue;
-    if (now.rows > 0 && p.ckpt) store_vec<float, VEC>(p.ckpt + (s.b * nck + now.ck) * p.D + s.d, in);
+    if (now.rows > 0 && p.ckpt) store_run<float, VEC>(p.ckpt + (s.b * nck + now.ck) * p.D + s.d, in);
     T* yp = y + (s.b * p.L + now.t0) * p.D + s.d;
     if (plain)
       write_states<true, T, VEC, K>(now, aa, uu, in, yp, p.D);
     else
       write_states<false, T, VEC, K>(now, aa, uu, in, yp, p.D);
   }
-  if (live && unit == 0 && s.seg == nseg - 1) store_vec<float, VEC>(p.h_last + s.b * p.D + s.d, carry);
+  if (live && unit == 0 && s.seg == nseg - 1) store_run<float, VEC>(p.h_last + s.b * p.D + s.d, carry);
 }
 
 // One chunk backward: z, 1 - z and the gate's factor dg / dh (cc) of each step, and the chunk's map of the state's
 // gradient. The gradients themselves follow in write_grads, from what enters the chunk.
 template <bool PLAIN, typename T, int VEC, int K>
-__device__ __forceinline__ void compose_back(const Chunk& c, const VecOf<T, VEC> (&x)[K], const VecOf<T, VEC> (&g)[K],
-                                             const VecOf<T, VEC> (&dy)[K], bool has_dy, float (&h)[VEC],
+__device__ __forceinline__ void compose_back(const Chunk& c, const RunOf<T, VEC> (&x)[K], const RunOf<T, VEC> (&g)[K],
+                                             const RunOf<T, VEC> (&dy)[K], bool has_dy, float (&h)[VEC],
                                              float (&zz)[K][VEC], float (&aa)[K][VEC], float (&cc)[K][VEC],
                                              Map (&m)[VEC]) {
 #pragma unroll
@@ -353,7 +355,7 @@ __device__ __forceinline__ void compose_back(const Chunk& c, const VecOf<T, VEC>
 }
 
 template <bool PLAIN, typename T, int VEC, int K>
-__device__ __forceinline__ void write_grads(const Chunk& c, const VecOf<T, VEC> (&dy)[K], bool has_dy,
+__device__ __forceinline__ void write_grads(const Chunk& c, const RunOf<T, VEC> (&dy)[K], bool has_dy,
                                             const float (&zz)[K][VEC], const float (&aa)[K][VEC],
                                             const float (&cc)[K][VEC], float (&in)[VEC], T* __restrict__ dx,
                                             T* __restrict__ dg, int64_t stride) {
@@ -369,8 +371,8 @@ __device__ __forceinline__ void write_grads(const Chunk& c, const VecOf<T, VEC> 
         og[v] = has ? d * cc[i][v] : 0.f;
         if (has) in[v] = drop ? 0.f : d * aa[i][v];
       }
-      store_vec<T, VEC>(dx + i * stride, ox);
-      store_vec<T, VEC>(dg + i * stride, og);
+      store_run<T, VEC>(dx + i * stride, ox);
+      store_run<T, VEC>(dg + i * stride, og);
     }
   }
 }
@@ -388,13 +390,13 @@ __global__ __launch_bounds__(kScanThreads) void k_scan_bwd(ScanArgs p, const T* 
   const int unit = s.wave * s.groups + s.group;
   const int first = (nseg - 1 - s.seg) * per, last = max(first + 1, min(first + per, (nck + units - 1) / units));
   const T *xp = x + s.b * p.xsb + s.d, *gp = g + s.b * p.gsb + s.d, *yp = dy ? dy + s.b * p.ysb + s.d : nullptr;
-  VecOf<T, VEC> xr[K], gr[K], yr[K];
+  RunOf<T, VEC> xr[K], gr[K], yr[K];
   float h[VEC] = {};
   Chunk c;
   const auto load = [&](int tile) {
     c = chunk_of<NARROW, K>(p, s, n, tile * units + unit);
     if (!live) return;
-    if (c.cnt > 0) load_vec<float, VEC>(p.ckpt + (s.b * nck + c.ck) * p.D + s.d, h);
+    if (c.cnt > 0) load_run<float, VEC>(p.ckpt + (s.b * nck + c.ck) * p.D + s.d, h);
     load_rows<T, VEC, K>(gp + c.t0 * p.gst, p.gst, c.cnt, gr);
     load_rows<T, VEC, K>(xp + c.t0 * p.xst, p.xst, c.cnt, xr);
     if (dy) load_rows<T, VEC, K>(yp + c.t0 * p.yst, p.yst, c.cnt, yr);
@@ -404,7 +406,7 @@ __global__ __launch_bounds__(kScanThreads) void k_scan_bwd(ScanArgs p, const T* 
   start_state<VEC>(p, s, s.seg, p.dh_last, seg_maps, carry);
   for (int tile = last - 1; tile >= first; tile--) {
     float zz[K][VEC], aa[K][VEC], cc[K][VEC], in[VEC];
-    VecOf<T, VEC> yn[K];
+    RunOf<T, VEC> yn[K];
     Map m[VEC];
     const Chunk now = c;
     const bool plain = is_plain<NARROW, K>(now) && dy != nullptr;
@@ -423,12 +425,12 @@ __global__ __launch_bounds__(kScanThreads) void k_scan_bwd(ScanArgs p, const T* 
     else
       write_grads<false, T, VEC, K>(now, yn, dy != nullptr, zz, aa, cc, in, dxp, dgp, p.dst);
   }
-  if (live && p.dh0 && unit == 0 && s.seg == nseg - 1) store_vec<float, VEC>(p.dh0 + s.b * p.D + s.d, carry);
+  if (live && p.dh0 && unit == 0 && s.seg == nseg - 1) store_run<float, VEC>(p.dh0 + s.b * p.D + s.d, carry);
 }
 
 // m becomes the chunk's map: forward of (gate, input), backward of (gate, dy).
 template <bool FORWARD, bool PLAIN, typename T, int VEC, int K>
-__device__ __forceinline__ void compose_map(const Chunk& c, const VecOf<T, VEC> (&g)[K], const VecOf<T, VEC> (&in)[K],
+__device__ __forceinline__ void compose_map(const Chunk& c, const RunOf<T, VEC> (&g)[K], const RunOf<T, VEC> (&in)[K],
                                             bool has_in, Map (&m)[VEC]) {
 #pragma unroll
   for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
@@ -480,7 +482,7 @@ __global__ __launch_bounds__(kMapWaves* kWave, NARROW || sizeof(T) == 4 ? 4 : 8)
     const int ck = FORWARD ? lo + k : hi - 1 - k;
     const Chunk c = chunk_of<NARROW, K>(p, s, NARROW && k >= hi - lo ? 0 : n, ck);
     if (!live || c.cnt == 0) continue;
-    VecOf<T, VEC> gr[K], ir[K];
+    RunOf<T, VEC> gr[K], ir[K];
     load_rows<T, VEC, K>(gp + c.t0 * p.gst, p.gst, c.cnt, gr);
     if (in) load_rows<T, VEC, K>(ip + c.t0 * ist, ist, c.cnt, ir);
     Map cm[VEC];
@@ -552,15 +554,6 @@ ScanPlan scan_plan(const ScanArgs& p, int type, int vec, const char* who) {
   return s;
 }
 
-// Two channels a lane where every row of every tensor starts at a multiple of two elements.
-template <typename T>
-bool pairs(const ScanArgs& p, std::initializer_list<const void*> ptrs) {
-  if ((p.D | p.xsb | p.xst | p.gsb | p.gst | p.ysb | p.yst | p.dsb | p.dst) % 2) return false;
-  for (const void* q : ptrs)
-    if (!vec_aligned<T, 2>(q)) return false;
-  return true;
-}
-
 template <typename T, int VEC, bool NARROW, bool FORWARD>
 void scan_maps_t(const ScanArgs& p, const ScanPlan& s, const T* g, const T* in, const char* who, hipStream_t stream) {
   if (s.nseg == 1) return;
@@ -595,7 +588,7 @@ int64_t gated_scan_workspace(int64_t B, int64_t L, int64_t D, int type) {
   ScanArgs p;
   p.B = B, p.L = L, p.D = D;
   if (B <= 0 || D <= 0) return 0;
-  const int nseg = std::max(scan_plan(p, type, 1, "gated_scan").nseg, scan_plan(p, type, 2, "gated_scan").nseg);
+  const int nseg = scan_plan(p, type, D > 1 ? 2 : 1, "gated_scan").nseg;
   return nseg == 1 ? 0 : (nseg - 1) * B * D * int64_t(sizeof(Map));
 }
 
@@ -603,7 +596,7 @@ void gated_scan_fwd(const ScanArgs& p, const void* x, const void* g, void* y, in
   if (p.B <= 0 || p.D <= 0) return;
   dispatch_type(type, "gated_scan", [&](auto tag) {
     using T = decltype(tag);
-    const int vec = pairs<T>(p, {x, g, y}) ? 2 : 1;
+    const int vec = p.D > 1 ? 2 : 1;
     const ScanPlan s = scan_plan(p, type, vec, "gated_scan");
     const auto fwd = vec == 2 ? (s.lpr < 6 ? scan_fwd_t<T, 2, true> : scan_fwd_t<T, 2, false>)
                               : (s.lpr < 6 ? scan_fwd_t<T, 1, true> : scan_fwd_t<T, 1, false>);
@@ -617,7 +610,7 @@ void gated_scan_bwd(const ScanArgs& p, const void* x, const void* g, const void*
   if (p.L > 0 && p.ckpt == nullptr) throw std::invalid_argument("gated_scan backward: no saved states");
   dispatch_type(type, "gated_scan backward", [&](auto tag) {
     using T = decltype(tag);
-    const int vec = pairs<T>(p, {x, g, dy, dx, dg}) ? 2 : 1;
+    const int vec = p.D > 1 ? 2 : 1;
     const ScanPlan s = scan_plan(p, type, vec, "gated_scan backward");
     const auto bwd = vec == 2 ? (s.lpr < 6 ? scan_bwd_t<T, 2, true> : scan_bwd_t<T, 2, false>)
                               : (s.lpr < 6 ? scan_bwd_t<T, 1, true> : scan_bwd_t<T, 1, false>);

@@ -64,6 +64,28 @@ inline bool vec_aligned(const void* p) {
   return reinterpret_cast<uintptr_t>(p) % alignof(VecOf<T, N>) == 0;
 }
 
+// N consecutive elements at any element's address: what gfx950 still reads and writes in one instruction for up to 16
+// bytes, whatever the alignment.
+template <typename T, int N>
+struct RunOf {
+  T v[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void load_run(const T* p, float (&x)[N]) {
+  const RunOf<T, N> r = *reinterpret_cast<const RunOf<T, N>*>(p);
+#pragma unroll
+  for (int k = 0; k < N; k++) x[k] = to_f32(r.v[k]);
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_run(T* p, const float (&x)[N]) {
+  RunOf<T, N> r;
+#pragma unroll
+  for (int k = 0; k < N; k++) r.v[k] = from_f32<T>(x[k]);
+  *reinterpret_cast<RunOf<T, N>*>(p) = r;
+}
+
 // Calls f(T{}) / f(A{}, B{}) for the element types of the codes.
 template <typename F>
 inline void dispatch_type(int t, const char* who, F&& f) {

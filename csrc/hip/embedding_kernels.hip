@@ -34,7 +34,11 @@ __device__ __forceinline__ uint32_t embed_key(TI id, int64_t V, int64_t pad) {
 }
 
 // ------------------------------------------------------------------------------------------ lookup
-// 2^lpr lanes share a row (VEC elements each, up to kRun times); a workgroup has 256 >> lpr rows in flight.
+// Everywhere below, a lane has VEC neighbouring columns at any alignment, and the last lane of a row whose length is no
+// multiple of VEC begins early enough to end with it: columns that two lanes have get the same value from both.
+__device__ __forceinline__ int64_t run_start(int64_t c, int64_t D, int vec) { return c + vec <= D ? c : D - vec; }
+
+// 2^lpr lanes share a row (up to kRun times); a workgroup has 256 >> lpr rows in flight.
 constexpr int kRun = 4;
 
 template <typename TI, typename TW, typename TO, int VEC>
@@ -48,17 +52,17 @@ __global__ __launch_bounds__(256) void k_embed_fwd(const TI* __restrict__ ids, c
   const bool ok = id >= 0 && id < V;
   const TW* row = w + (ok ? id : 0) * ws;
   for (int64_t c0 = int64_t(lane) * VEC; c0 < D; c0 += kRun * step) {
-    VecOf<TW, VEC> r[kRun];
+    RunOf<TW, VEC> r[kRun];
 #pragma unroll
     for (int q = 0; q < kRun; q++)
-      if (ok && c0 + q * step < D) r[q] = *reinterpret_cast<const VecOf<TW, VEC>*>(row + c0 + q * step);
+      if (ok && c0 + q * step < D) r[q] = *reinterpret_cast<const RunOf<TW, VEC>*>(row + run_start(c0 + q * step, D, VEC));
 #pragma unroll
     for (int q = 0; q < kRun; q++) {
       if (c0 + q * step >= D) break;
       float v[VEC];
 #pragma unroll
       for (int k = 0; k < VEC; k++) v[k] = ok ? to_f32(r[q].v[k]) * scale : 0.f;
-      store_vec<TO, VEC>(out + i * D + c0 + q * step, v);
+      store_run<TO, VEC>(out + i * D + run_start(c0 + q * step, D, VEC), v);
     }
   }
 }
@@ -312,7 +316,7 @@ __device__ __forceinline__ void write_row(TW* __restrict__ dw, int64_t at, const
   float o[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; k++) o[k] = acc[k] * scale;
-  store_vec<TW, VEC>(dw + at, o);
+  store_run<TW, VEC>(dw + at, o);
 }
 
 template <typename TW, typename TO, int VEC>
@@ -333,14 +337,15 @@ __global__ __launch_bounds__(256) void k_embed_sum(const uint32_t* __restrict__ 
     const int lane = threadIdx.x & ((1 << s.lpr) - 1);
     for (int r = threadIdx.x >> s.lpr; r < rows; r += 256 >> s.lpr) {
       if (used[r]) continue;
-      for (int64_t c = int64_t(lane) * VEC; c < D; c += int64_t(VEC) << s.lpr) store_vec<TW, VEC>(dw + (v0 + r) * D + c, zero);
+      for (int64_t c = int64_t(lane) * VEC; c < D; c += int64_t(VEC) << s.lpr) store_run<TW, VEC>(dw + (v0 + r) * D + run_start(c, D, VEC), zero);
     }
     return;
   }
   const int64_t unit = (int64_t(blockIdx.x) * 256 + threadIdx.x) >> s.lpr;
   const int64_t p = unit / s.chunks;
-  const int64_t c = ((unit - p * s.chunks) << s.lpr) * VEC + (threadIdx.x & ((1 << s.lpr) - 1)) * VEC;
-  if (p >= s.pieces || c >= D) return;
+  const int64_t c0 = ((unit - p * s.chunks) << s.lpr) * VEC + (threadIdx.x & ((1 << s.lpr) - 1)) * VEC;
+  if (p >= s.pieces || c0 >= D) return;
+  const int64_t c = run_start(c0, D, VEC);
   const uint32_t lo = uint32_t(p * s.piece), hi = uint32_t(min(int64_t(n), int64_t(lo) + s.piece));
   uint32_t cur = keys[lo];
   bool entered = lo > 0 && keys[lo - 1] == cur;  // the segment at hand began in an earlier piece
@@ -348,19 +353,19 @@ __global__ __launch_bounds__(256) void k_embed_sum(const uint32_t* __restrict__ 
   float acc[VEC] = {};
   for (uint32_t j0 = lo; j0 < hi; j0 += kAhead) {
     uint32_t k[kAhead];
-    VecOf<TO, VEC> row[kAhead];
+    RunOf<TO, VEC> row[kAhead];
 #pragma unroll
     for (int q = 0; q < kAhead; q++) {
       const uint32_t j = min(j0 + q, hi - 1);
       k[q] = keys[j];
-      row[q] = *reinterpret_cast<const VecOf<TO, VEC>*>(dy + int64_t(pos[j]) * dys + c);
+      row[q] = *reinterpret_cast<const RunOf<TO, VEC>*>(dy + int64_t(pos[j]) * dys + c);
     }
 #pragma unroll
     for (int q = 0; q < kAhead; q++) {
       if (j0 + q >= hi) break;
       if (k[q] != cur) {
         if (entered) {
-          store_vec<float, VEC>(part + 2 * p * D + c, acc);
+          store_run<float, VEC>(part + 2 * p * D + c, acc);
         } else {
           write_row<TW, VEC>(dw, int64_t(cur) * D + c, acc, scale);
         }
@@ -375,7 +380,7 @@ __global__ __launch_bounds__(256) void k_embed_sum(const uint32_t* __restrict__ 
     }
   }
   if (entered || leaves)
-    store_vec<float, VEC>(part + (2 * p + (entered ? 0 : 1)) * D + c, acc);
+    store_run<float, VEC>(part + (2 * p + (entered ? 0 : 1)) * D + c, acc);
   else
     write_row<TW, VEC>(dw, int64_t(cur) * D + c, acc, scale);
 }
@@ -402,8 +407,8 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void k_embed_join(const uint32_t
     count += got;
     more = got == kWave;
   }
-  const int64_t c = ((ch << s.lpr) + lane) * VEC;
-  const bool live = lane < (1 << s.lpr) && c < D;
+  const int64_t c0 = ((ch << s.lpr) + lane) * VEC, c = run_start(c0, D, VEC);
+  const bool live = lane < (1 << s.lpr) && c0 < D;
   const int64_t per = (count + kJoinWaves - 1) / kJoinWaves, q0 = min(count, wave * per), q1 = min(count, q0 + per);
   float acc[VEC] = {};
   if (live) {
@@ -411,7 +416,7 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void k_embed_join(const uint32_t
 #pragma unroll 16
     for (int64_t q = q0; q < q1; q++) {
       float x[VEC];
-      load_vec<float, VEC>(part + (2 * (p + q) + (q == 0 ? 1 : 0)) * D + c, x);
+      load_run<float, VEC>(part + (2 * (p + q) + (q == 0 ? 1 : 0)) * D + c, x);
 #pragma unroll
       for (int e = 0; e < VEC; e++) acc[e] += x[e];
     }
@@ -481,16 +486,16 @@ void embed_fwd_t(const TI* ids, const void* w, int64_t ws, void* out, int64_t n,
   TO* op = static_cast<TO*>(out);
   const auto run = [&](auto width) {
     constexpr int VEC = decltype(width)::value;
-    if (D % VEC || ws % VEC || !vec_aligned<TW, VEC>(w) || !vec_aligned<TO, VEC>(out)) return false;
     // a wave a row where there are rows enough to fill the card, else up to a workgroup a row
     const int lpr = std::min(lanes_log2(D, VEC), n >= 4096 ? 6 : 8);
     hipLaunchKernelGGL((k_embed_fwd<TI, TW, TO, VEC>), dim3(row_blocks(n, lpr, "embedding")), dim3(256), 0, stream, ids,
                        wp, ws, op, n, V, D, scale, lpr);
     RMM_HIP_CHECK(hipGetLastError());
-    return true;
   };
-  using std::integral_constant;  // the widest rows that the sizes and addresses allow
-  run(integral_constant<int, 8>{}) || run(integral_constant<int, 2>{}) || run(integral_constant<int, 1>{});
+  if (D >= 8)
+    run(std::integral_constant<int, 8>{});
+  else
+    run(std::integral_constant<int, 1>{});
 }
 
 template <typename TI>
@@ -540,19 +545,13 @@ void embed_sum_t(const uint32_t* keys, const uint32_t* pos, int64_t n, const TO*
   RMM_HIP_CHECK(hipGetLastError());
 }
 
-// 16 bytes of dy a lane where the rows allow it, else pairs, else single elements.
+// 16 bytes of dy a lane, or single elements of rows shorter than that.
 template <typename TW, typename TO>
 void embed_sum_any(const uint32_t* keys, const uint32_t* pos, int64_t n, const void* dy, int64_t dys, void* dw,
                    float* part, int64_t V, int64_t D, float scale, hipStream_t stream) {
   constexpr int VEC = 16 / sizeof(TO);
-  const TO* yp = static_cast<const TO*>(dy);
-  TW* wp = static_cast<TW*>(dw);
-  if (D % VEC == 0 && dys % VEC == 0 && vec_aligned<TO, VEC>(dy) && vec_aligned<TW, VEC>(dw))
-    embed_sum_t<TW, TO, VEC>(keys, pos, n, yp, dys, wp, part, V, D, scale, stream);
-  else if (D % 2 == 0 && dys % 2 == 0 && vec_aligned<TO, 2>(dy) && vec_aligned<TW, 2>(dw))
-    embed_sum_t<TW, TO, 2>(keys, pos, n, yp, dys, wp, part, V, D, scale, stream);
-  else
-    embed_sum_t<TW, TO, 1>(keys, pos, n, yp, dys, wp, part, V, D, scale, stream);
+  const auto sum = D >= VEC ? embed_sum_t<TW, TO, VEC> : embed_sum_t<TW, TO, 1>;
+  sum(keys, pos, n, static_cast<const TO*>(dy), dys, static_cast<TW*>(dw), part, V, D, scale, stream);
 }
 
 }  // namespace
@@ -573,7 +572,7 @@ void embedding_fwd(const void* ids, bool ids64, const void* w, int wtype, int64_
 int64_t embedding_grad_workspace(int64_t n, int64_t V, int64_t D) {
   if (n <= 0 || D <= 0) return 0;
   int64_t pieces = 0;  // of whichever width the launch will have
-  for (int vec : {8, 4, 2, 1}) pieces = std::max(pieces, sum_plan(n, D, vec, vec >= 4).pieces);
+  for (int vec : {8, 4, 1}) pieces = std::max(pieces, sum_plan(n, D, vec, vec >= 4).pieces);
   return (sort_words(n, V) + 3) / 4 * 16 + (pieces > 1 ? 2 * pieces * D * int64_t(sizeof(float)) : 0);
 }
 

@@ -44,7 +44,7 @@ __device__ __forceinline__ Philox4 philox10(uint64_t index, uint64_t offset, uin
   return Philox4{{a, b, c, d}};
 }
 
-template <typename T, bool RES, bool WIDE>
+template <typename T, bool RES>
 __global__ __launch_bounds__(256) void k_dropout(const T* __restrict__ x, const T* __restrict__ res, T* __restrict__ out,
                                                  int64_t n, uint32_t t, float scale, uint64_t seed, uint64_t offset,
                                                  const int64_t* __restrict__ ctr, int64_t* __restrict__ used) {
@@ -56,9 +56,9 @@ __global__ __launch_bounds__(256) void k_dropout(const T* __restrict__ x, const 
   const Philox4 r = philox10(uint64_t(q), off, seed);
   float v[8], s[8];
   const int m = int(n - i < 8 ? n - i : 8);
-  if (WIDE && m == 8) {
-    load_vec<T, 8>(x + i, v);
-    if (RES) load_vec<T, 8>(res + i, s);
+  if (m == 8) {
+    load_run<T, 8>(x + i, v);
+    if (RES) load_run<T, 8>(res + i, s);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; k++) {
@@ -72,8 +72,8 @@ __global__ __launch_bounds__(256) void k_dropout(const T* __restrict__ x, const 
     v[k] = u >= t ? v[k] * scale : 0.f;  // a select: what is dropped is zero whatever it held
     if (RES) v[k] += s[k];
   }
-  if (WIDE && m == 8) {
-    store_vec<T, 8>(out + i, v);
+  if (m == 8) {
+    store_run<T, 8>(out + i, v);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; k++)
@@ -93,21 +93,9 @@ void dropout(const void* x, const void* res, void* out, int type, int64_t n, dou
   if (blocks > (int64_t(1) << 31) - 1) throw std::invalid_argument("dropout: too many elements");
   dispatch_type(type, "dropout", [&](auto tag) {
     using T = decltype(tag);
-    const bool wide = vec_aligned<T, 8>(x) && vec_aligned<T, 8>(out) && vec_aligned<T, 8>(res);
-    const T *xp = static_cast<const T*>(x), *rp = static_cast<const T*>(res);
-    T* op = static_cast<T*>(out);
-    const dim3 grid{uint32_t(blocks)}, block{256};
-#define RMM_DROP(R, W) \
-  hipLaunchKernelGGL((k_dropout<T, R, W>), grid, block, 0, stream, xp, rp, op, n, t, scale, seed, offset, ctr, used)
-    if (res && wide)
-      RMM_DROP(true, true);
-    else if (res)
-      RMM_DROP(true, false);
-    else if (wide)
-      RMM_DROP(false, true);
-    else
-      RMM_DROP(false, false);
-#undef RMM_DROP
+    const auto kernel = res ? k_dropout<T, true> : k_dropout<T, false>;
+    hipLaunchKernelGGL(kernel, dim3(uint32_t(blocks)), dim3(256), 0, stream, static_cast<const T*>(x),
+                       static_cast<const T*>(res), static_cast<T*>(out), n, t, scale, seed, offset, ctr, used);
   });
   RMM_HIP_CHECK(hipGetLastError());
 }

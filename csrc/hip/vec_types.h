@@ -38,32 +38,6 @@ __device__ __forceinline__ bf16_t from_f32<bf16_t>(float v) {
   return bf16_t{__builtin_bit_cast(uint16_t, r)};
 }
 
-// N consecutive elements starting at a multiple of min(16, N * size) bytes (any N = 1, 2, 4, 8).
-template <typename T, int N>
-struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) VecOf {
-  T v[N];
-};
-
-template <typename T, int N>
-__device__ __forceinline__ void load_vec(const T* p, float (&x)[N]) {
-  const VecOf<T, N> r = *reinterpret_cast<const VecOf<T, N>*>(p);
-#pragma unroll
-  for (int k = 0; k < N; k++) x[k] = to_f32(r.v[k]);
-}
-
-template <typename T, int N>
-__device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
-  VecOf<T, N> r;
-#pragma unroll
-  for (int k = 0; k < N; k++) r.v[k] = from_f32<T>(x[k]);
-  *reinterpret_cast<VecOf<T, N>*>(p) = r;
-}
-
-template <typename T, int N>
-inline bool vec_aligned(const void* p) {
-  return reinterpret_cast<uintptr_t>(p) % alignof(VecOf<T, N>) == 0;
-}
-
 // N consecutive elements at any element's address: what gfx950 still reads and writes in one instruction for up to 16
 // bytes, whatever the alignment.
 template <typename T, int N>

@@ -213,11 +213,17 @@ __device__ __forceinline__ Chunk chunk_of(const ScanArgs& p, const ScanPlace& s,
   return c;
 }
 
-// Whether the chunk's steps all take part, without a reset, in every lane.
+// Whether the chunk is PLAIN, which has code of its own: all K steps take part, and none has a reset. In a wave of
+// several chunks some chunk nearly always has a reset, so that there PLAIN allows them: testing whether each step takes
+// part is what costs.
 template <bool NARROW, int K>
 __device__ __forceinline__ bool is_plain(const Chunk& c) {
-  const bool plain = c.cnt == K && c.resets == 0;
-  return NARROW ? __all(plain) : plain;
+  return NARROW ? __all(c.cnt == K) : c.cnt == K && c.resets == 0;
+}
+
+template <bool PLAIN, bool NARROW>
+__device__ __forceinline__ bool drops(const Chunk& c, int i) {
+  return (NARROW || !PLAIN) && ((c.resets >> i) & 1);
 }
 
 // The chunk's factor of the state before it, from the plain product of its steps' factors.
@@ -225,15 +231,15 @@ __device__ __forceinline__ float chunk_factor(const Chunk& c, float product) {
   return c.resets ? 0.f : fmaxf(product, kTiny);
 }
 
-// One chunk forward: 1 - z and z x of each step, and the chunk's map. PLAIN: all K steps and no reset.
-template <bool PLAIN, typename T, int VEC, int K>
+// One chunk forward: 1 - z and z x of each step, and the chunk's map.
+template <bool PLAIN, bool NARROW, typename T, int VEC, int K>
 __device__ __forceinline__ void compose(const Chunk& c, const RunOf<T, VEC> (&x)[K], const RunOf<T, VEC> (&g)[K],
                                         float (&aa)[K][VEC], float (&uu)[K][VEC], Map (&m)[VEC]) {
 #pragma unroll
   for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
 #pragma unroll
   for (int i = 0; i < K; i++) {
-    const bool drop = !PLAIN && ((c.resets >> i) & 1);
+    const bool drop = drops<PLAIN, NARROW>(c, i);
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
       if (PLAIN || i < c.cnt) {
@@ -249,13 +255,13 @@ __device__ __forceinline__ void compose(const Chunk& c, const RunOf<T, VEC> (&x)
   for (int v = 0; v < VEC; v++) m[v].A = chunk_factor(c, m[v].A);
 }
 
-template <bool PLAIN, typename T, int VEC, int K>
+template <bool PLAIN, bool NARROW, typename T, int VEC, int K>
 __device__ __forceinline__ void write_states(const Chunk& c, const float (&aa)[K][VEC], const float (&uu)[K][VEC],
                                              float (&h)[VEC], T* __restrict__ y, int64_t stride) {
 #pragma unroll
   for (int i = 0; i < K; i++) {
     if (PLAIN || i < c.rows) {
-      const bool drop = !PLAIN && ((c.resets >> i) & 1), has = PLAIN || i < c.cnt;
+      const bool drop = drops<PLAIN, NARROW>(c, i), has = PLAIN || i < c.cnt;
       float o[VEC];
 #pragma unroll
       for (int v = 0; v < VEC; v++) {
@@ -294,9 +300,9 @@ __global__ __launch_bounds__(kScanThreads, NARROW ? 2 : 4) void k_scan_fwd(ScanA
     const Chunk now = c;
     const bool plain = is_plain<NARROW, K>(now);
     if (plain)
-      compose<true, T, VEC, K>(now, xr, gr, aa, uu, m);
+      compose<true, NARROW, T, VEC, K>(now, xr, gr, aa, uu, m);
     else
-      compose<false, T, VEC, K>(now, xr, gr, aa, uu, m);
+      compose<false, NARROW, T, VEC, K>(now, xr, gr, aa, uu, m);
     if (tile + 1 < last) {
       c = chunk_of<NARROW, K>(p, s, n, (tile + 1) * units + unit);
       if (live) {
@@ -309,16 +315,16 @@ __global__ __launch_bounds__(kScanThreads, NARROW ? 2 : 4) void k_scan_fwd(ScanA
     if (now.rows > 0 && p.ckpt) store_run<float, VEC>(p.ckpt + (s.b * nck + now.ck) * p.D + s.d, in);
     T* yp = y + (s.b * p.L + now.t0) * p.D + s.d;
     if (plain)
-      write_states<true, T, VEC, K>(now, aa, uu, in, yp, p.D);
+      write_states<true, NARROW, T, VEC, K>(now, aa, uu, in, yp, p.D);
     else
-      write_states<false, T, VEC, K>(now, aa, uu, in, yp, p.D);
+      write_states<false, NARROW, T, VEC, K>(now, aa, uu, in, yp, p.D);
   }
   if (live && unit == 0 && s.seg == nseg - 1) store_run<float, VEC>(p.h_last + s.b * p.D + s.d, carry);
 }
 
 // One chunk backward: z, 1 - z and the gate's factor dg / dh (cc) of each step, and the chunk's map of the state's
 // gradient. The gradients themselves follow in write_grads, from what enters the chunk.
-template <bool PLAIN, typename T, int VEC, int K>
+template <bool PLAIN, bool NARROW, typename T, int VEC, int K>
 __device__ __forceinline__ void compose_back(const Chunk& c, const RunOf<T, VEC> (&x)[K], const RunOf<T, VEC> (&g)[K],
                                              const RunOf<T, VEC> (&dy)[K], bool has_dy, float (&h)[VEC],
                                              float (&zz)[K][VEC], float (&aa)[K][VEC], float (&cc)[K][VEC],
@@ -327,7 +333,7 @@ __device__ __forceinline__ void compose_back(const Chunk& c, const RunOf<T, VEC>
   for (int v = 0; v < VEC; v++) m[v] = Map{1.f, 0.f};
 #pragma unroll
   for (int i = 0; i < K; i++) {
-    const bool drop = !PLAIN && ((c.resets >> i) & 1);
+    const bool drop = drops<PLAIN, NARROW>(c, i);
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
       if (PLAIN || i < c.cnt) {
@@ -340,7 +346,7 @@ __device__ __forceinline__ void compose_back(const Chunk& c, const RunOf<T, VEC>
   }
 #pragma unroll
   for (int i = K - 1; i >= 0; i--) {
-    const bool drop = !PLAIN && ((c.resets >> i) & 1);
+    const bool drop = drops<PLAIN, NARROW>(c, i);
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
       if (PLAIN || i < c.cnt) {
@@ -354,7 +360,7 @@ __device__ __forceinline__ void compose_back(const Chunk& c, const RunOf<T, VEC>
   for (int v = 0; v < VEC; v++) m[v].A = chunk_factor(c, m[v].A);
 }
 
-template <bool PLAIN, typename T, int VEC, int K>
+template <bool PLAIN, bool NARROW, typename T, int VEC, int K>
 __device__ __forceinline__ void write_grads(const Chunk& c, const RunOf<T, VEC> (&dy)[K], bool has_dy,
                                             const float (&zz)[K][VEC], const float (&aa)[K][VEC],
                                             const float (&cc)[K][VEC], float (&in)[VEC], T* __restrict__ dx,
@@ -362,7 +368,7 @@ __device__ __forceinline__ void write_grads(const Chunk& c, const RunOf<T, VEC> 
 #pragma unroll
   for (int i = K - 1; i >= 0; i--) {
     if (PLAIN || i < c.rows) {
-      const bool drop = !PLAIN && ((c.resets >> i) & 1), has = PLAIN || i < c.cnt;
+      const bool drop = drops<PLAIN, NARROW>(c, i), has = PLAIN || i < c.cnt;
       float ox[VEC], og[VEC];
 #pragma unroll
       for (int v = 0; v < VEC; v++) {
@@ -411,9 +417,9 @@ __global__ __launch_bounds__(kScanThreads) void k_scan_bwd(ScanArgs p, const T* 
     const Chunk now = c;
     const bool plain = is_plain<NARROW, K>(now) && dy != nullptr;
     if (plain)
-      compose_back<true, T, VEC, K>(now, xr, gr, yr, true, h, zz, aa, cc, m);
+      compose_back<true, NARROW, T, VEC, K>(now, xr, gr, yr, true, h, zz, aa, cc, m);
     else
-      compose_back<false, T, VEC, K>(now, xr, gr, yr, dy != nullptr, h, zz, aa, cc, m);
+      compose_back<false, NARROW, T, VEC, K>(now, xr, gr, yr, dy != nullptr, h, zz, aa, cc, m);
 #pragma unroll
     for (int i = 0; i < K; i++) yn[i] = yr[i];
     if (tile > first) load(tile - 1);
@@ -421,15 +427,15 @@ __global__ __launch_bounds__(kScanThreads) void k_scan_bwd(ScanArgs p, const T* 
     if (!live) continue;
     T *dxp = dx + s.b * p.dsb + now.t0 * p.dst + s.d, *dgp = dg + s.b * p.dsb + now.t0 * p.dst + s.d;
     if (plain)
-      write_grads<true, T, VEC, K>(now, yn, true, zz, aa, cc, in, dxp, dgp, p.dst);
+      write_grads<true, NARROW, T, VEC, K>(now, yn, true, zz, aa, cc, in, dxp, dgp, p.dst);
     else
-      write_grads<false, T, VEC, K>(now, yn, dy != nullptr, zz, aa, cc, in, dxp, dgp, p.dst);
+      write_grads<false, NARROW, T, VEC, K>(now, yn, dy != nullptr, zz, aa, cc, in, dxp, dgp, p.dst);
   }
   if (live && p.dh0 && unit == 0 && s.seg == nseg - 1) store_run<float, VEC>(p.dh0 + s.b * p.D + s.d, carry);
 }
 
 // m becomes the chunk's map: forward of (gate, input), backward of (gate, dy).
-template <bool FORWARD, bool PLAIN, typename T, int VEC, int K>
+template <bool FORWARD, bool PLAIN, bool NARROW, typename T, int VEC, int K>
 __device__ __forceinline__ void compose_map(const Chunk& c, const RunOf<T, VEC> (&g)[K], const RunOf<T, VEC> (&in)[K],
                                             bool has_in, Map (&m)[VEC]) {
 #pragma unroll
@@ -437,7 +443,7 @@ __device__ __forceinline__ void compose_map(const Chunk& c, const RunOf<T, VEC> 
 #pragma unroll
   for (int q = 0; q < K; q++) {
     const int i = FORWARD ? q : K - 1 - q;
-    const bool drop = !PLAIN && ((c.resets >> i) & 1);
+    const bool drop = drops<PLAIN, NARROW>(c, i);
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
       if (PLAIN || i < c.cnt) {
@@ -486,10 +492,10 @@ __global__ __launch_bounds__(kMapWaves* kWave, NARROW || sizeof(T) == 4 ? 4 : 8)
     load_rows<T, VEC, K>(gp + c.t0 * p.gst, p.gst, c.cnt, gr);
     if (in) load_rows<T, VEC, K>(ip + c.t0 * ist, ist, c.cnt, ir);
     Map cm[VEC];
-    if (c.cnt == K && c.resets == 0 && in)
-      compose_map<FORWARD, true, T, VEC, K>(c, gr, ir, true, cm);
+    if (is_plain<NARROW, K>(c) && in)
+      compose_map<FORWARD, true, NARROW, T, VEC, K>(c, gr, ir, true, cm);
     else
-      compose_map<FORWARD, false, T, VEC, K>(c, gr, ir, in != nullptr, cm);
+      compose_map<FORWARD, false, NARROW, T, VEC, K>(c, gr, ir, in != nullptr, cm);
 #pragma unroll
     for (int v = 0; v < VEC; v++) m[v] = then(m[v], cm[v]);
   }

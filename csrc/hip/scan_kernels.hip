@@ -18,7 +18,7 @@
 // tile of chunks with the state behind this one, whose loads they issued before the exchange. With enough chains (one
 // sequence's 64 VEC channels) to fill the card, that reads x, g (and dy) once. With fewer, a chain is cut into segments:
 // k_scan_maps composes the map of each from a first reading, and the workgroups of the pass itself start from the maps
-// before theirs. Rows narrower than half a wave's reach put several chunks into a wave.
+// before theirs. Rows narrower than half a wave's reach put several chunks into a wave. VEC is 2 at any alignment.
 //
 // Bound by memory, x, g, dy and the outputs crossing the bus once (twice for the inputs where chains are cut): bf16, us and
 // TB/s, forward / backward: [1024, 64, 1024] 78 (5.2) / 141 (4.8), [32, 2048, 1024] 89 (4.5) / 150 (4.5),

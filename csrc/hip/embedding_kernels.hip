@@ -55,7 +55,8 @@ __global__ __launch_bounds__(256) void k_embed_fwd(const TI* __restrict__ ids, c
     RunOf<TW, VEC> r[kRun];
 #pragma unroll
     for (int q = 0; q < kRun; q++)
-      if (ok && c0 + q * step < D) r[q] = *reinterpret_cast<const RunOf<TW, VEC>*>(row + run_start(c0 + q * step, D, VEC));
+      if (ok && c0 + q * step < D)
+        r[q] = *reinterpret_cast<const RunOf<TW, VEC>*>(row + run_start(c0 + q * step, D, VEC));
 #pragma unroll
     for (int q = 0; q < kRun; q++) {
       if (c0 + q * step >= D) break;
@@ -337,7 +338,8 @@ __global__ __launch_bounds__(256) void k_embed_sum(const uint32_t* __restrict__ 
     const int lane = threadIdx.x & ((1 << s.lpr) - 1);
     for (int r = threadIdx.x >> s.lpr; r < rows; r += 256 >> s.lpr) {
       if (used[r]) continue;
-      for (int64_t c = int64_t(lane) * VEC; c < D; c += int64_t(VEC) << s.lpr) store_run<TW, VEC>(dw + (v0 + r) * D + run_start(c, D, VEC), zero);
+      for (int64_t c = int64_t(lane) * VEC; c < D; c += int64_t(VEC) << s.lpr)
+        store_run<TW, VEC>(dw + (v0 + r) * D + run_start(c, D, VEC), zero);
     }
     return;
   }
@@ -472,7 +474,7 @@ SumPlan sum_plan(int64_t n, int64_t D, int vec, bool wide) {
   SumPlan s;
   s.lpr = std::min(6, lanes_log2(D, vec));
   s.chunks = (D + (int64_t(vec) << s.lpr) - 1) / (int64_t(vec) << s.lpr);
-  const int64_t lanes = s.chunks << s.lpr, waves = wide ? 1536 : 3072;
+  const int64_t lanes = s.chunks << s.lpr, waves = wide ? 1500 : 3000;
   s.piece = 16;
   while (s.piece < 256 && n / (2 * s.piece) * lanes >= waves * kWave) s.piece *= 2;
   s.pieces = (n + s.piece - 1) / s.piece;

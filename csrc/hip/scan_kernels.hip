@@ -275,9 +275,10 @@ __device__ __forceinline__ void write_states(const Chunk& c, const float (&aa)[K
 
 // `per` tiles in a segment.
 template <typename T, int VEC, bool NARROW>
-__global__ __launch_bounds__(kScanThreads, NARROW ? 2 : 4) void k_scan_fwd(ScanArgs p, const T* __restrict__ x, const T* __restrict__ g,
-                                                              T* __restrict__ y, int nseg, int per, int lpr,
-                                                              const Map* __restrict__ seg_maps) {
+__global__ __launch_bounds__(kScanThreads, NARROW ? 2 : 4) void k_scan_fwd(ScanArgs p, const T* __restrict__ x,
+                                                                            const T* __restrict__ g, T* __restrict__ y,
+                                                                            int nseg, int per, int lpr,
+                                                                            const Map* __restrict__ seg_maps) {
   constexpr int K = chunk_steps<T>();
   __shared__ Map maps[2][kScanWaves][kWave * VEC];
   const ScanPlace s = scan_place<VEC, NARROW>(p, lpr);
@@ -468,9 +469,9 @@ __device__ __forceinline__ void compose_map(const Chunk& c, const RunOf<T, VEC> 
 constexpr int kMapWaves = 16;
 
 template <typename T, int VEC, bool NARROW, bool FORWARD>
-__global__ __launch_bounds__(kMapWaves* kWave, NARROW || sizeof(T) == 4 ? 4 : 8) void k_scan_maps(ScanArgs p, const T* __restrict__ g,
-                                                                   const T* __restrict__ in, int nseg, int len,
-                                                                   int lpr, Map* __restrict__ seg_maps) {
+__global__ __launch_bounds__(kMapWaves* kWave, NARROW || sizeof(T) == 4 ? 4 : 8) void k_scan_maps(
+    ScanArgs p, const T* __restrict__ g, const T* __restrict__ in, int nseg, int len, int lpr,
+    Map* __restrict__ seg_maps) {
   constexpr int K = chunk_steps<T>();
   __shared__ Map maps[kMapWaves][kWave * VEC];
   const ScanPlace s = scan_place<VEC, NARROW>(p, lpr);

@@ -622,3 +622,21 @@ def test_a_token_model_trains_through_all_three(dev):
     assert abs(got_loss - want_loss) < 4096 * U * want_loss
     for a, b in zip(got[1], want[1]):
         assert float((a.cpu().double() - b).abs().max()) < 4096 * U * float(b.abs().max())
+
+
+def test_gated_scan_with_some_gradients_wanted(dev):
+    """Any subset of the inputs may want gradients, and one tensor may be both input and gate."""
+    x, g, h0 = (rand(*s, seed=k).to(dev) for k, s in enumerate(((2, 9, 6), (2, 9, 6), (2, 6))))
+    full = [v.clone().requires_grad_() for v in (x, g, h0)]
+    y, h = ops.gated_scan(*full)
+    want = torch.autograd.grad(y.sum() + h.sum(), full)
+    for k in range(3):
+        ins = [v.clone().requires_grad_(i == k) for i, v in enumerate((x, g, h0))]
+        y, h = ops.gated_scan(*ins)
+        assert torch.equal(torch.autograd.grad(y.sum() + h.sum(), ins[k])[0], want[k])
+    both = x.clone().requires_grad_()
+    y, h = ops.gated_scan(both, both)
+    (got,) = torch.autograd.grad(y.sum() + h.sum(), both)
+    two = [x.clone().requires_grad_() for _ in range(2)]
+    y, h = ops.gated_scan(*two)
+    assert torch.equal(got, sum(torch.autograd.grad(y.sum() + h.sum(), two)))

@@ -12,12 +12,12 @@ import torch
 
 from ray_memory_management_amd._native import hip_ext, require_hip
 from ray_memory_management_amd.ops.sequence import (Dropout, Embedding, dropout, embedding, gated_scan,
-                                                    gated_scan_step)
+                                                    gated_scan_step, repeatable)
 
 __all__ = [
     "multi_copy", "pack_tensors", "unpack_tensors", "concat", "gather_rows", "gae", "vtrace",
     "compress", "decompress", "ppo_loss", "hip_available", "embedding", "Embedding", "dropout", "Dropout", "gated_scan",
-    "gated_scan_step",
+    "gated_scan_step", "repeatable",
 ]
 
 

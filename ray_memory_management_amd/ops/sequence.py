@@ -17,7 +17,7 @@ from torch.autograd.function import once_differentiable
 
 from ray_memory_management_amd._native import require_seq
 
-__all__ = ["embedding", "Embedding", "dropout", "Dropout", "gated_scan", "gated_scan_step"]
+__all__ = ["embedding", "Embedding", "dropout", "Dropout", "repeatable", "gated_scan", "gated_scan_step"]
 
 _CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # the type codes of the kernels
 
@@ -144,7 +144,8 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: Union[int, torch.Tenso
 
     offset: the call's own number under the seed: an int, or an int64 tensor on x's device whose first element is read
     when the kernel runs (a graph replay then draws a new mask after each advance); the backward pass uses the value
-    that its forward pass read. residual: same shape and type as x."""
+    that its forward pass read. A call that activation checkpointing repeats reads the tensor again: there, give it one
+    that stays as it is until the backward pass. residual: same shape and type as x."""
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout: p must be in [0, 1], not {p}")
     if residual is not None:
@@ -169,10 +170,21 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: Union[int, torch.Tenso
     return require_seq().dropout(x, residual, p, seed, offset, ctr)
 
 
+def _in_backward() -> bool:
+    """Whether this thread runs a backward pass, which calls layers only to recompute what they gave."""
+    return torch._C._current_graph_task_id() != -1
+
+
 class Dropout(nn.Module):
     """Dropout layer over :func:`dropout`. Its call counter is a buffer on the layer's device that every training call
     advances there, so a captured graph draws a new mask on each replay and a restored state dict goes on where it was
-    saved. Layers of one model take different seeds."""
+    saved. Masks follow from the seed and the counter alone: layers of one model take different seeds, and so do the
+    ranks of a data-parallel group.
+
+    Activation checkpointing calls the layer again in the backward pass, when the counter has moved on. Checkpoint
+    ``ops.repeatable(block)`` in place of ``block``; without it the second call raises."""
+
+    _repeats = 0  # above 0 while :class:`repeatable` has set the counter back
 
     def __init__(self, p: float = 0.5, seed: int = 0):
         super().__init__()
@@ -184,12 +196,51 @@ class Dropout(nn.Module):
     def forward(self, x, residual=None):
         if not self.training or self.p == 0.0:
             return dropout(x, self.p, self.seed, residual=residual, training=False)
+        if not self._repeats and _in_backward():
+            raise RuntimeError("Dropout: called again in a backward pass, where its counter has moved on and would draw "
+                               "another mask: checkpoint ops.repeatable(block) in place of the block")
         y = dropout(x, self.p, self.seed, self.counter, residual)
         self.counter.add_(1)
         return y
 
     def extra_repr(self):
         return f"p={self.p}, seed={self.seed}"
+
+
+class repeatable:
+    """``fn`` for one checkpointed call, ``checkpoint(ops.repeatable(block), x)``, with either ``use_reentrant``.
+
+    The first call notes the counters of the :class:`Dropout` layers in ``fn``; the later ones, of the recomputation,
+    start from these and leave the layers as they were, so they draw the masks of the first. modules: where the layers
+    are if ``fn`` is no module itself. Each checkpointed call takes a wrapper of its own."""
+
+    def __init__(self, fn, *modules: nn.Module):
+        roots = [m for m in (fn, *modules) if isinstance(m, nn.Module)]
+        if not roots:
+            raise ValueError("repeatable: fn is no module: name the modules whose Dropout layers it calls")
+        self.fn, self.start = fn, None
+        self.layers = list({id(m): m for r in roots for m in r.modules() if isinstance(m, Dropout)}.values())
+
+    def __call__(self, *args, **kw):
+        again = _in_backward()
+        if self.start is None:
+            if again and not all(m._repeats for m in self.layers):
+                raise RuntimeError("repeatable: first called in a backward pass: the region around it has to be "
+                                   "repeatable too")
+            self.start = [m.counter.clone() for m in self.layers]
+            return self.fn(*args, **kw)
+        if not again:
+            raise RuntimeError("repeatable: each checkpointed call takes a wrapper of its own")
+        now = [m.counter.clone() for m in self.layers]
+        for m, start in zip(self.layers, self.start):
+            m.counter.copy_(start)
+            m._repeats += 1
+        try:
+            return self.fn(*args, **kw)
+        finally:
+            for m, c in zip(self.layers, now):
+                m.counter.copy_(c)
+                m._repeats -= 1
 
 
 # ------------------------------------------------------------------------------------------ gated scan

@@ -56,6 +56,12 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 
+// The kernels carry no tangents: a dual tensor is refused, with or without requires_grad.
+void refuse_tangents(const char* who, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), who, ": no forward-mode derivatives on the GPU");
+}
+
 // Inside a graph's capture, a leaf whose gradient accumulator an eager graph on the default stream keeps alive would have
 // the captured backward pass wait on that stream, which ends the process. Said here instead.
 void check_capture(std::initializer_list<const Tensor*> leaves) {
@@ -72,7 +78,8 @@ void check_capture(std::initializer_list<const Tensor*> leaves) {
 
 // Gradients that say so when they are differentiated again. Only a pass with create_graph runs with gradients enabled.
 template <typename F>
-variable_list first_order(F&& compute) {
+variable_list first_order(const char* who, const variable_list& grads, F&& compute) {
+  for (const Tensor& g : grads) refuse_tangents(who, {&g});
   if (!at::GradMode::is_enabled()) return compute();
   variable_list out;
   {
@@ -113,7 +120,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const Tensor ids = ctx->get_saved_variables()[0];
-    return first_order([&]() -> variable_list {
+    return first_order("embedding backward", grads, [&]() -> variable_list {
       const c10::DeviceGuard guard(ids.device());
       const int64_t n = ids.numel(), V = ctx->saved_data["rows"].toInt(), D = ctx->saved_data["cols"].toInt();
       const Tensor dy = rows(grads[0].reshape({n, D}));
@@ -128,6 +135,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
 };
 
 Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, int64_t pad, int64_t type) {
+  refuse_tangents("embedding", {&weight});
   const Tensor i = ids.contiguous();
   if (!wants_grad({&weight})) return embedding_run(i, weight, scale, type_of(type));
   check_capture({&weight});
@@ -161,7 +169,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const Tensor used = ctx->get_saved_variables()[0];
-    return first_order([&]() -> variable_list {
+    return first_order("dropout backward", grads, [&]() -> variable_list {
       Tensor dx;
       if (ctx->needs_input_grad(0))
         dx = dropout_run(grads[0], Tensor(), ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(),
@@ -173,6 +181,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 
 Tensor dropout(const Tensor& x, const OptTensor& res, double p, uint64_t seed, uint64_t offset, const OptTensor& ctr) {
   const Tensor r = plain(res);
+  refuse_tangents("dropout", {&x, &r});
   if (!wants_grad({&x, &r})) return dropout_run(x, r, p, int64_t(seed), int64_t(offset), plain(ctr), Tensor());
   check_capture({&x, &r});
   return Dropout::apply(x, res, p, int64_t(seed), int64_t(offset), ctr);
@@ -234,7 +243,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list saved = ctx->get_saved_variables();
-    return first_order([&]() -> variable_list {
+    return first_order("gated_scan backward", grads, [&]() -> variable_list {
       const Tensor &x = saved[0], &gate = saved[1], &ckpt = saved[4];
       const c10::DeviceGuard guard(x.device());
       ScanCall c(x, gate, saved[2], saved[3]);
@@ -267,11 +276,13 @@ OptTensor flags(const OptTensor& resets) {
 
 std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const OptTensor& gate, const OptTensor& h0, const OptTensor& resets,
                                       const OptTensor& lengths) {
+  const Tensor g = plain(gate), first = plain(h0);
+  refuse_tangents("gated_scan", {&x, &g, &first});
   OptTensor h, n;
   if (h0) h = h0->to(at::kFloat).contiguous();
   if (lengths) n = lengths->to(at::kLong).contiguous();
   const OptTensor r = flags(resets);
-  const Tensor g = plain(gate), state = plain(h);
+  const Tensor state = plain(h);
   if (!wants_grad({&x, &g, &state})) {
     auto [y, last, ckpt] = scan_run(rows(x), gate ? rows(g) : g, state, plain(r), plain(n), false);
     return {y, last};
@@ -283,6 +294,8 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const OptTensor& gate, co
 
 std::tuple<Tensor, Tensor> gated_scan_step(const Tensor& x, const OptTensor& gate, const Tensor& state,
                                            const OptTensor& resets, const OptTensor& out) {
+  const Tensor gt = plain(gate), ot = plain(out);
+  refuse_tangents("gated_scan_step", {&x, &gt, &state, &ot});
   const c10::DeviceGuard guard(x.device());
   const Tensor xr = rows(x), g = gate ? rows(*gate) : Tensor(), r = plain(flags(resets));
   const int64_t B = state.size(0), D = state.size(1);

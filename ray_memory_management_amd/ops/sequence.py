@@ -6,6 +6,7 @@ CUDA(ROCm) tensors run the HIP kernels on the current stream of their device; CP
 fp32, bf16 and fp16 are taken on the GPU; sums and states are held in fp32. Everything here can be captured into a
 graph: nothing synchronises, and what a call keeps for its backward pass belongs to that call. (A capture refuses leaves
 that a graph made outside it still holds: torch's engine would have the captured backward pass wait on their stream.)
+Second and forward-mode derivatives are refused on the GPU.
 """
 from __future__ import annotations
 

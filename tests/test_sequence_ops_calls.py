@@ -127,3 +127,33 @@ def test_a_recomputed_layer_in_a_graph(cuda):
         torch.cuda.synchronize()
         assert torch.equal(y, ops.dropout(src, 0.5, 3, at + k)) and torch.equal(g, y)
     assert int(m.counter) == at + 4
+
+
+# ------------------------------------------------------------------------------------------ derivatives
+@pytest.mark.gpu
+def test_forward_mode_derivatives_are_refused(cuda):
+    """A dual tensor without requires_grad would come out without its tangent."""
+    import torch.autograd.forward_ad as fw
+
+    def both(*shape):
+        v = torch.randn(*shape, device=cuda)
+        return v, fw.make_dual(v.clone(), torch.ones_like(v))
+
+    with fw.dual_level():
+        (x, xd), (w, wd), (h, hd) = both(2, 5, 8), both(6, 8), both(2, 8)
+        ids = torch.zeros(3, dtype=torch.long, device=cuda)
+        calls = [lambda: ops.embedding(ids, wd), lambda: ops.dropout(xd, 0.5, 1), lambda: ops.dropout(x, 0.5, 1, residual=xd),
+                 lambda: ops.gated_scan(xd, x), lambda: ops.gated_scan(x, xd), lambda: ops.gated_scan(xd),
+                 lambda: ops.gated_scan(x, x, hd), lambda: ops.gated_scan(x, x, hd.requires_grad_()),
+                 lambda: ops.gated_scan_step(xd[:, 0], x[:, 0], h), lambda: ops.gated_scan_step(x[:, 0], x[:, 0], hd)]
+        for call in calls:
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+            with pytest.raises((NotImplementedError, ValueError), match="forward-mode|not differentiable"):
+                call()
+        dy = fw.make_dual(torch.ones(2, 5, 8, device=cuda), torch.ones(2, 5, 8, device=cuda))
+        leaf, table = x.clone().requires_grad_(), w.clone().requires_grad_()
+        for y in (ops.dropout(leaf, 0.5, 1), ops.gated_scan(leaf, x)[0], ops.embedding(ids.new_zeros(2, 5), table)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                y.backward(dy)
+    ops.gated_scan(x, x, h)  # outside the level nothing is refused

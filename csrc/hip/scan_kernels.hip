@@ -27,7 +27,7 @@
 // arithmetic that these times leave room for; fp32 tensors have chunks of 8 steps to keep within the registers.
 //
 // A = 0 stands for a reset alone: what is before it is dropped, not multiplied by zero (it may be infinite or NaN).
-// Products that underflow are held at the smallest denormal instead, so an infinite state stays infinite.
+// Factors and products that underflow are held at the smallest denormal instead, so an infinite state stays infinite.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -50,12 +50,19 @@ constexpr int chunk_steps() {
   return sizeof(T) == 4 ? 8 : 16;
 }
 
-// z = sigmoid(g) and a = 1 - z, both to full relative precision: from exp(-|g|), which cannot overflow.
-__device__ __forceinline__ void gate_of(float g, float& z, float& a) {
+// z = sigmoid(g) and a = 1 - z from exp(-|g|), which cannot overflow: within about |g| + 8 roundings (the exponent's own
+// grows with it). Above 87 the smaller of them is zero, though for a finite gate it is not: the recurrence takes the smallest
+// denormal more, at no cost, so that an infinite state or input stays infinite. The gradients' factors do without it.
+struct Gate {
+  float z, a;
+  float dx, dg;  // z and z (1 - z)
+};
+
+__device__ __forceinline__ Gate gate_of(float g) {
   const float e = __expf(-fabsf(g));
-  const float big = __builtin_amdgcn_rcpf(1.f + e), small = e * big;
-  z = g >= 0.f ? big : small;
-  a = g >= 0.f ? small : big;
+  const float big = __builtin_amdgcn_rcpf(1.f + e), small = e * big, held = fmaf(e, big, kTiny);
+  const bool open = g >= 0.f;
+  return Gate{open ? big : held, open ? held : big, open ? big : small, big * small};
 }
 
 __device__ __forceinline__ int length_of(const int64_t* __restrict__ lengths, int64_t b, int L) {
@@ -243,9 +250,9 @@ __device__ __forceinline__ void compose(const Chunk& c, const RunOf<T, VEC> (&x)
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
       if (PLAIN || i < c.cnt) {
-        float z;
-        gate_of(to_f32(g[i].v[v]), z, aa[i][v]);
-        uu[i][v] = z * to_f32(x[i].v[v]);
+        const Gate q = gate_of(to_f32(g[i].v[v]));
+        aa[i][v] = q.a;
+        uu[i][v] = q.z * to_f32(x[i].v[v]);
         m[v].H = drop ? uu[i][v] : fmaf(aa[i][v], m[v].H, uu[i][v]);
         m[v].A *= aa[i][v];
       }
@@ -338,10 +345,11 @@ __device__ __forceinline__ void compose_back(const Chunk& c, const RunOf<T, VEC>
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
       if (PLAIN || i < c.cnt) {
-        gate_of(to_f32(g[i].v[v]), zz[i][v], aa[i][v]);
+        const Gate q = gate_of(to_f32(g[i].v[v]));
+        zz[i][v] = q.dx, aa[i][v] = q.a;
         const float xv = to_f32(x[i].v[v]), prev = drop ? 0.f : h[v];
-        cc[i][v] = (xv - prev) * (zz[i][v] * aa[i][v]);
-        h[v] = fmaf(aa[i][v], prev, zz[i][v] * xv);
+        cc[i][v] = (xv - prev) * q.dg;
+        h[v] = fmaf(q.a, prev, q.z * xv);
       }
     }
   }
@@ -448,14 +456,13 @@ __device__ __forceinline__ void compose_map(const Chunk& c, const RunOf<T, VEC> 
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
       if (PLAIN || i < c.cnt) {
-        float z, a;
-        gate_of(to_f32(g[i].v[v]), z, a);
+        const Gate gt = gate_of(to_f32(g[i].v[v]));
         const float iv = PLAIN || has_in ? to_f32(in[i].v[v]) : 0.f;
         if (FORWARD)
-          m[v].H = drop ? z * iv : fmaf(a, m[v].H, z * iv);
+          m[v].H = drop ? gt.z * iv : fmaf(gt.a, m[v].H, gt.z * iv);
         else
-          m[v].H = drop ? 0.f : a * (m[v].H + iv);
-        m[v].A *= a;
+          m[v].H = drop ? 0.f : gt.a * (m[v].H + iv);
+        m[v].A *= gt.a;
       }
     }
   }
@@ -523,10 +530,9 @@ __global__ __launch_bounds__(256) void k_scan_step(const T* __restrict__ x, int6
   const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (i >= B * D) return;
   const int64_t b = i / D, d = i - b * D;
-  float z, a;
-  gate_of(to_f32(g[b * gs + d]), z, a);
-  const float u = z * to_f32(x[b * xs + d]);
-  const float hn = resets && resets[b] ? u : fmaf(a, h[i], u);
+  const Gate q = gate_of(to_f32(g[b * gs + d]));
+  const float u = q.z * to_f32(x[b * xs + d]);
+  const float hn = resets && resets[b] ? u : fmaf(q.a, h[i], u);
   out[i] = hn;
   y[i] = from_f32<T>(hn);
 }

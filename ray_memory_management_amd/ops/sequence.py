@@ -245,21 +245,27 @@ class repeatable:
 
 
 # ------------------------------------------------------------------------------------------ gated scan
+def _held(v):
+    """A sigmoid, a little more than zero also where the type has none for it: for a finite gate it is not zero, and zero
+    times an infinite state or input would be NaN."""
+    return v.clamp(min=torch.finfo(v.dtype).smallest_normal * torch.finfo(v.dtype).eps)
+
+
 class _Gate(torch.autograd.Function):
-    """sigmoid(g) and 1 - sigmoid(g) with their relative precision on both sides, in the gradient too (that of
-    torch.sigmoid takes 1 - z by a subtraction, which has none left near z = 1)."""
+    """The step's factor 1 - z of the state and its share z x of the input, z = sigmoid(g), with their relative precision on
+    both sides, in the gradient too (that of torch.sigmoid takes 1 - z by a subtraction, which has none left near z = 1)."""
 
     @staticmethod
-    def forward(ctx, g):
+    def forward(ctx, g, x):
         z, a = torch.sigmoid(g), torch.sigmoid(-g)
-        ctx.save_for_backward(z, a)
-        return z, a
+        ctx.save_for_backward(z, a, x)
+        return _held(a), _held(z) * x
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dz, da):
-        z, a = ctx.saved_tensors
-        return (dz - da) * z * a
+    def backward(ctx, da, du):
+        z, a, x = ctx.saved_tensors
+        return (du * x - da) * z * a, du * z
 
 
 def _scan_cpu(x, gate, h0, resets, lengths):
@@ -271,11 +277,11 @@ def _scan_cpu(x, gate, h0, resets, lengths):
     if lengths is not None:
         live = (torch.arange(L) < lengths.unsqueeze(1)).unsqueeze(-1)
         x, gate = torch.where(live, x, zero), torch.where(live, gate, zero)
-    z, a = _Gate.apply(gate)
+    a, u = _Gate.apply(gate, x)
     ys = []
     for t in range(L):
         prev = h if resets is None else torch.where((resets != 0)[:, t, None], torch.zeros((), dtype=st), h)
-        new = a[:, t] * prev + z[:, t] * x[:, t]
+        new = a[:, t] * prev + u[:, t]
         h = new if live is None else torch.where(live[:, t], new, h)
         ys.append(new if live is None else torch.where(live[:, t], new, torch.zeros((), dtype=new.dtype)))
     return (torch.stack(ys, dim=1) if L else x.new_zeros((B, 0, D), dtype=st)), h
@@ -308,8 +314,10 @@ def gated_scan(x: torch.Tensor, gate: Optional[torch.Tensor] = None, h0: Optiona
     x, gate: same shape and type; any strides with consecutive channels are read in place. Without ``gate``, x is
     [B, L, 2D], inputs and gates in its halves as one projection gives them, and so is its gradient.
     h0: [B, D] state before the first step (zeros by default). resets: [B, L], non-zero where the state is dropped
-    before the step (an episode or document begins). lengths: [B] integers, steps of each sequence (clamped to
-    [0, L]): later places take no part whatever they hold, their y and gradients are 0."""
+    before the step (an episode or document begins), whatever it held. Without one, an infinite state stays infinite under
+    any gate (an infinite gate counts as a very large one).
+    lengths: [B] integers, steps of each sequence (clamped to [0, L]): later places take no part whatever they hold, their
+    y and gradients are 0."""
     D = _scan_parts("gated_scan", x, gate)
     B, L = x.shape[:2]
     _same_device("gated_scan", x, gate=gate, h0=h0, resets=resets, lengths=lengths)
@@ -355,7 +363,7 @@ def gated_scan_step(x: torch.Tensor, gate: Optional[torch.Tensor], state: torch.
         if gate is None:
             x, gate = x[..., :D], x[..., D:]
         prev = state if resets is None else torch.where((resets != 0).unsqueeze(-1), torch.zeros(()), state)
-        h = torch.sigmoid(-gate.float()) * prev + torch.sigmoid(gate.float()) * x.float()
+        h = _held(torch.sigmoid(-gate.float())) * prev + _held(torch.sigmoid(gate.float())) * x.float()
         out = h if out is None else out.copy_(h)
         return out.to(x.dtype, copy=True), out
     _code("gated_scan_step", x.dtype)

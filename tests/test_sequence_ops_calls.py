@@ -157,3 +157,84 @@ def test_forward_mode_derivatives_are_refused(cuda):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 y.backward(dy)
     ops.gated_scan(x, x, h)  # outside the level nothing is refused
+
+
+# ------------------------------------------------------------------------------------------ gates that are fully open
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("L,D", [(40, 1), (40, 2), (300, 64), (700, 20), (2500, 130)])
+def test_an_open_gate_under_an_infinite_state(dev, L, D, t):
+    """1 - sigmoid(200) is e^-200, zero in fp32 and yet not zero: by the recurrence an infinite state stays infinite, in
+    both directions, wherever in a chunk, a tile or a segment the step falls, until a reset."""
+    at = torch.arange(L, device=dev)[:, None]
+    p = (10 + 13 * torch.arange(D, device=dev) % (L - 25))[None]  # a step a channel
+    gate = torch.where(at == p, 200.0, 0.0).to(t)[None]
+    reset = L - 6
+    for with_reset in (False, True):
+        resets = torch.zeros(1, L, dtype=torch.bool, device=dev)
+        resets[0, reset] = with_reset
+        x = torch.zeros(1, L, D, dtype=t, device=dev)
+        x[0, 3] = float("inf")
+        y, h = ops.gated_scan(x, gate, resets=resets)
+        live = ((at >= 3) & ~((at >= reset) & with_reset)).expand(L, D)
+        assert (y[0][live] == float("inf")).all() and (y[0][~live] == 0).all()
+        assert (h == (0 if with_reset else float("inf"))).all()
+        # the gradient of the state goes the other way, and meets the reset first
+        resets = torch.zeros(1, L, dtype=torch.bool, device=dev)
+        resets[0, 4] = with_reset
+        x = torch.ones(1, L, D, dtype=t, device=dev, requires_grad=True)
+        h0 = torch.ones(1, D, device=dev, requires_grad=True)
+        y, h = ops.gated_scan(x, gate, h0, resets=resets)
+        dy = torch.zeros_like(y)
+        dy[0, L - 5] = float("inf")
+        dx, dh0 = torch.autograd.grad(y, (x, h0), dy)
+        live = ((at <= L - 5) & ~((at < 4) & with_reset)).expand(L, D)
+        assert (dx[0][live] == float("inf")).all() and (dx[0][~live] == 0).all()
+        assert (dh0 == (0 if with_reset else float("inf"))).all()
+
+
+@pytest.mark.parametrize("g", [87.0, 88.0, 95.0, 103.0, 104.0, 200.0, 700.0])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_open_and_closed_gates_match_the_recurrence_in_64_bits(dev, g, sign):
+    """Sequence k has an infinite input at step k in channel 2; the first three an infinite first state. 64 bits hold e^-g."""
+    L = 40
+    x, gate = torch.zeros(L, L, 3), torch.full((L, L, 3), 0.5)
+    x[torch.arange(L), torch.arange(L), 2] = float("inf")
+    gate[:, 17] = gate[:, 23] = sign * g
+    h0 = torch.diag(torch.full((L,), float("inf")))[:, :3].contiguous()
+    y, h = (v.cpu() for v in ops.gated_scan(x.to(dev), gate.to(dev), h0.to(dev)))
+    state, want = h0.double(), []
+    for k in range(L):
+        state = torch.sigmoid(-gate[:, k].double()) * state + torch.sigmoid(gate[:, k].double()) * x[:, k].double()
+        want.append(state)
+    want = torch.stack(want, 1)
+    assert torch.equal(y.isinf(), want.isinf()) and torch.equal(h.isinf(), state.isinf())
+    assert not y.isnan().any() and not h.isnan().any()
+    ys, hs = (v.cpu() for v in ops.gated_scan_step(x[:, 17].to(dev), gate[:, 17].to(dev), h0.to(dev)))
+    assert torch.equal(hs.isinf(), h0.isinf() | x[:, 17].isinf()) and torch.equal(ys, hs) and not hs.isnan().any()
+
+
+def test_open_gates_leave_next_to_nothing_of_a_state(dev):
+    """A finite state behind one is the input's; a gate or input that is NaN stays NaN until a reset."""
+    for L, D in ((40, 2), (600, 64)):
+        gate = torch.zeros(1, L, D, device=dev)
+        gate[0, 20] = float("inf")
+        y, h = ops.gated_scan(torch.zeros_like(gate), gate, torch.ones(1, D, device=dev))
+        assert (y[0, :20] > 0).all() and (y[0, 20:] <= 1.5e-45).all() and (h <= 1.5e-45).all()
+        gate[0, 20] = float("nan")
+        resets = torch.zeros(1, L, device=dev)
+        resets[0, 30] = 1
+        y, h = ops.gated_scan(torch.zeros_like(gate), gate, torch.ones(1, D, device=dev), resets=resets)
+        assert y[0, 20:30].isnan().all() and not y[0, :20].isnan().any() and (y[0, 30:] == 0).all() and (h == 0).all()
+        resets[0, 30], resets[0, 20] = 0, 1  # a NaN gate at the reset itself
+        y, h = ops.gated_scan(torch.ones_like(gate), gate, torch.ones(1, D, device=dev), resets=resets)
+        assert y[0, 20:].isnan().all() and h.isnan().all()
+
+
+def test_products_that_underflow_keep_an_infinite_state(dev):
+    """400 steps of 1 - z = e^-20 leave an infinite state infinite, forward and backward."""
+    x = torch.zeros(1, 400, 3, device=dev, requires_grad=True)
+    h0 = torch.full((1, 3), float("inf"), device=dev, requires_grad=True)
+    y, h = ops.gated_scan(x, torch.full((1, 400, 3), 20.0, device=dev), h0)
+    assert y.isinf().all() and h.isinf().all()
+    (dx,) = torch.autograd.grad(h, x, torch.full_like(h, float("inf")))
+    assert dx.isinf().all()

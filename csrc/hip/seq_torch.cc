@@ -287,7 +287,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const OptTensor& gate, co
     auto [y, last, ckpt] = scan_run(rows(x), gate ? rows(g) : g, state, plain(r), plain(n), false);
     return {y, last};
   }
-  check_capture({&x, &g, &state});
+  check_capture({&x, &g, &first});  // h0 itself: its fp32 copy is no leaf
   const variable_list out = GatedScan::apply(x, gate, h, r, n);
   return {out[0], out[1]};
 }

@@ -159,6 +159,29 @@ def test_forward_mode_derivatives_are_refused(cuda):
     ops.gated_scan(x, x, h)  # outside the level nothing is refused
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["half", "apart"])
+def test_a_capture_over_a_first_state_of_a_living_graph_is_refused(cuda, kind):
+    """Also where the call makes an fp32 copy of h0, which is no leaf."""
+    h0 = torch.ones(2, 4, dtype=torch.half, device=cuda) if kind == "half" else torch.ones(4, 2, device=cuda).t()
+    h0 = h0.detach().requires_grad_()
+    x = torch.zeros(2, 3, 4, device=cuda)
+    alive = ops.gated_scan(x, x, h0)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="outside the capture"):
+        with torch.cuda.graph(graph):
+            ops.gated_scan(x, x, h0)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, h = ops.gated_scan(x, x, h0)
+        (g,) = torch.autograd.grad(h, h0, torch.ones_like(h))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (g == 0.125).all() and (h == 0.125).all() and g.dtype == h0.dtype
+
+
 # ------------------------------------------------------------------------------------------ gates that are fully open
 @pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("L,D", [(40, 1), (40, 2), (300, 64), (700, 20), (2500, 130)])

@@ -292,12 +292,23 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const OptTensor& gate, co
   return {out[0], out[1]};
 }
 
+// Whether the memory that a and b span meets (a with any strides that are not negative, b contiguous).
+bool meets(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  int64_t last = 0;
+  for (int64_t d = 0; d < a.dim(); d++) last += (a.size(d) - 1) * a.stride(d);
+  const char *a0 = static_cast<const char*>(a.data_ptr()), *b0 = static_cast<const char*>(b.data_ptr());
+  return a0 < b0 + b.nbytes() && b0 < a0 + (last + 1) * a.element_size();
+}
+
 std::tuple<Tensor, Tensor> gated_scan_step(const Tensor& x, const OptTensor& gate, const Tensor& state,
                                            const OptTensor& resets, const OptTensor& out) {
   const Tensor gt = plain(gate), ot = plain(out);
   refuse_tangents("gated_scan_step", {&x, &gt, &state, &ot});
   const c10::DeviceGuard guard(x.device());
-  const Tensor xr = rows(x), g = gate ? rows(*gate) : Tensor(), r = plain(flags(resets));
+  // a lane reads its own inputs before it writes its state, but not those of others: inputs under `out` are copied
+  const auto apart = [&](const Tensor& t) { return ot.defined() && t.defined() && meets(t, ot) ? t.clone() : t; };
+  const Tensor xr = apart(rows(x)), g = apart(gate ? rows(*gate) : Tensor()), r = apart(plain(flags(resets)));
   const int64_t B = state.size(0), D = state.size(1);
   Tensor to = out ? *out : made(state.sizes(), state, at::kFloat), y = made({B, D}, x, x.scalar_type());
   const void* gp = g.defined() ? ptr(g) : static_cast<char*>(ptr(xr)) + D * xr.element_size();

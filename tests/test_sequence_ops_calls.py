@@ -182,6 +182,30 @@ def test_a_capture_over_a_first_state_of_a_living_graph_is_refused(cuda, kind):
         assert (g == 0.125).all() and (h == 0.125).all() and g.dtype == h0.dtype
 
 
+# ------------------------------------------------------------------------------------------ a step's out
+def test_a_step_into_its_own_inputs(dev):
+    """out over x, over the packed projection, over the gate, over the resets: as with an out of its own."""
+    B, D = 64, 1024
+    src = torch.randn(B, 2 * D, generator=torch.Generator().manual_seed(0))
+    state = torch.randn(B, D, generator=torch.Generator().manual_seed(1)).to(dev)
+    flags = (torch.rand(B, generator=torch.Generator().manual_seed(2)) < 0.3).to(dev)
+    y, h = ops.gated_scan_step(src.to(dev), None, state, flags)
+    for at in (0, 512, B * D):
+        buf = src.clone().to(dev)
+        ya, ha = ops.gated_scan_step(buf, None, state, flags, out=buf.view(-1)[at:at + B * D].view(B, D))
+        assert torch.equal(ya, y) and torch.equal(ha, h)
+    x, g = (v.contiguous().to(dev) for v in src.chunk(2, -1))
+    for k in range(2):
+        xs = [x.clone(), g.clone()]
+        ya, ha = ops.gated_scan_step(*xs, state, flags, out=xs[k])
+        assert ha is xs[k] and torch.equal(ya, y) and torch.equal(ha, h)
+    buf = torch.empty(B, D, device=dev)
+    bits = buf.view(-1)[-B:].view(torch.uint8)[:B].view(torch.bool)
+    bits.copy_(flags)
+    ya, ha = ops.gated_scan_step(x, g, state, bits, out=buf)
+    assert torch.equal(ya, y) and torch.equal(ha, h)
+
+
 # ------------------------------------------------------------------------------------------ gates that are fully open
 @pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("L,D", [(40, 1), (40, 2), (300, 64), (700, 20), (2500, 130)])

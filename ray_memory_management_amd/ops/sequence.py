@@ -351,7 +351,7 @@ def gated_scan_step(x: torch.Tensor, gate: Optional[torch.Tensor], state: torch.
     for name, t in (("state", state), ("out", out)):
         if t is not None and (tuple(t.shape) != (B, D) or t.dtype != torch.float32 or not t.is_contiguous()):
             raise ValueError(f"gated_scan_step: {name} must be {(B, D)}, fp32 and contiguous")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, state)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, state, out)):
         raise ValueError("gated_scan_step is not differentiable: call gated_scan with L = 1, or under torch.no_grad()")
     if out is not None:
         delta = abs(out.data_ptr() - state.data_ptr())

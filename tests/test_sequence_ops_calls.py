@@ -206,6 +206,16 @@ def test_a_step_into_its_own_inputs(dev):
     assert torch.equal(ya, y) and torch.equal(ha, h)
 
 
+def test_a_step_into_what_wants_gradients_is_refused(dev):
+    z = torch.zeros(2, 4, device=dev)
+    leaf = torch.zeros(2, 4, device=dev, requires_grad=True)
+    for out in (leaf, leaf * 1.0):
+        with pytest.raises(ValueError, match="not differentiable"):
+            ops.gated_scan_step(z, z, z, out=out)
+    with torch.no_grad():
+        ops.gated_scan_step(z, z, z, out=leaf)
+
+
 # ------------------------------------------------------------------------------------------ gates that are fully open
 @pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("L,D", [(40, 1), (40, 2), (300, 64), (700, 20), (2500, 130)])

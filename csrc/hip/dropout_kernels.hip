@@ -90,11 +90,11 @@ void dropout(const void* x, const void* res, void* out, int type, int64_t n, dou
   const uint32_t t = uint32_t(std::nearbyint(p * 65536.0));
   const float scale = t < 65536u ? float(65536.0 / double(65536u - t)) : 0.f;
   const int64_t blocks = (n + 2047) / 2048;
-  if (blocks > (int64_t(1) << 31) - 1) throw std::invalid_argument("dropout: too many elements");
+  const dim3 grid = grid_of(blocks, 256, "dropout", "elements");
   dispatch_type(type, "dropout", [&](auto tag) {
     using T = decltype(tag);
     const auto kernel = res ? k_dropout<T, true> : k_dropout<T, false>;
-    hipLaunchKernelGGL(kernel, dim3(uint32_t(blocks)), dim3(256), 0, stream, static_cast<const T*>(x),
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, static_cast<const T*>(x),
                        static_cast<const T*>(res), static_cast<T*>(out), n, t, scale, seed, offset, ctr, used);
   });
   RMM_HIP_CHECK(hipGetLastError());

@@ -301,7 +301,8 @@ struct SumPlan {
 };
 
 constexpr int kAhead = 8;        // rows of dy in flight per lane
-constexpr int kZeroRows = 64;    // rows that a zero-writing workgroup looks at
+constexpr int kZeroRows = 64;    // rows that a zero-writing workgroup looks at at a time
+constexpr int64_t kZeroGroups = 1 << 22;  // such workgroups at most: they go on in steps of all of them
 
 __device__ __forceinline__ uint32_t lower_bound(const uint32_t* __restrict__ keys, uint32_t n, uint32_t v) {
   uint32_t lo = 0, hi = n;
@@ -327,19 +328,22 @@ __global__ __launch_bounds__(256) void k_embed_sum(const uint32_t* __restrict__ 
                                                    float scale, SumPlan s, uint32_t sum_blocks) {
   if (blockIdx.x >= sum_blocks) {
     __shared__ bool used[kZeroRows];
-    const int64_t v0 = int64_t(blockIdx.x - sum_blocks) * kZeroRows;
-    const int rows = int(min(int64_t(kZeroRows), V - v0));
-    if (threadIdx.x < rows) {
-      const uint32_t v = uint32_t(v0 + threadIdx.x), at = lower_bound(keys, n, v);
-      used[threadIdx.x] = at < n && keys[at] == v;
-    }
-    __syncthreads();
     float zero[VEC] = {};
     const int lane = threadIdx.x & ((1 << s.lpr) - 1);
-    for (int r = threadIdx.x >> s.lpr; r < rows; r += 256 >> s.lpr) {
-      if (used[r]) continue;
-      for (int64_t c = int64_t(lane) * VEC; c < D; c += int64_t(VEC) << s.lpr)
-        store_run<TW, VEC>(dw + (v0 + r) * D + run_start(c, D, VEC), zero);
+    const int64_t step = int64_t(gridDim.x - sum_blocks) * kZeroRows;
+    for (int64_t v0 = int64_t(blockIdx.x - sum_blocks) * kZeroRows; v0 < V; v0 += step) {
+      const int rows = int(min(int64_t(kZeroRows), V - v0));
+      if (threadIdx.x < rows) {
+        const uint32_t v = uint32_t(v0 + threadIdx.x), at = lower_bound(keys, n, v);
+        used[threadIdx.x] = at < n && keys[at] == v;
+      }
+      __syncthreads();
+      for (int r = threadIdx.x >> s.lpr; r < rows; r += 256 >> s.lpr) {
+        if (used[r]) continue;
+        for (int64_t c = int64_t(lane) * VEC; c < D; c += int64_t(VEC) << s.lpr)
+          store_run<TW, VEC>(dw + (v0 + r) * D + run_start(c, D, VEC), zero);
+      }
+      __syncthreads();
     }
     return;
   }
@@ -441,12 +445,6 @@ int lanes_log2(int64_t D, int vec) {
   return lpr;
 }
 
-uint32_t row_blocks(int64_t rows, int lpr, const char* who) {
-  const int64_t blocks = (rows + (256 >> lpr) - 1) / (256 >> lpr);
-  if (blocks > (int64_t(1) << 31) - 1) throw std::invalid_argument(std::string(who) + ": too many rows");
-  return uint32_t(blocks);
-}
-
 struct SortPlan {
   bool small = false;
   int64_t tile = 0;
@@ -488,10 +486,11 @@ void embed_fwd_t(const TI* ids, const void* w, int64_t ws, void* out, int64_t n,
   TO* op = static_cast<TO*>(out);
   const auto run = [&](auto width) {
     constexpr int VEC = decltype(width)::value;
-    // a wave a row where there are rows enough to fill the card, else up to a workgroup a row
-    const int lpr = std::min(lanes_log2(D, VEC), n >= 4096 ? 6 : 8);
-    hipLaunchKernelGGL((k_embed_fwd<TI, TW, TO, VEC>), dim3(row_blocks(n, lpr, "embedding")), dim3(256), 0, stream, ids,
-                       wp, ws, op, n, V, D, scale, lpr);
+    // a wave a row where there are rows enough to fill the card, else up to a workgroup a row; less where n passes a launch
+    int lpr = std::min(lanes_log2(D, VEC), n >= 4096 ? 6 : 8);
+    while (lpr > 0 && (n << lpr) > (int64_t(1) << 31)) lpr--;
+    const dim3 grid = grid_of((n + (256 >> lpr) - 1) / (256 >> lpr), 256, "embedding", "ids");
+    hipLaunchKernelGGL((k_embed_fwd<TI, TW, TO, VEC>), grid, dim3(256), 0, stream, ids, wp, ws, op, n, V, D, scale, lpr);
     RMM_HIP_CHECK(hipGetLastError());
   };
   if (D >= 8)
@@ -537,13 +536,14 @@ template <typename TW, typename TO, int VEC>
 void embed_sum_t(const uint32_t* keys, const uint32_t* pos, int64_t n, const TO* dy, int64_t dys, TW* dw, float* part,
                  int64_t V, int64_t D, float scale, hipStream_t stream) {
   const SumPlan s = sum_plan(n, D, VEC, VEC * sizeof(TO) >= 16);
-  const int64_t sums = ((s.pieces * s.chunks << s.lpr) + 255) / 256, zeros = (V + kZeroRows - 1) / kZeroRows;
-  if (sums + zeros > (int64_t(1) << 31) - 1) throw std::invalid_argument("embedding_grad: too many elements");
-  hipLaunchKernelGGL((k_embed_sum<TW, TO, VEC>), dim3(uint32_t(sums + zeros)), dim3(256), 0, stream, keys, pos,
-                     uint32_t(n), dy, dys, dw, part, V, D, scale, s, uint32_t(sums));
+  const int64_t sums = ((s.pieces * s.chunks << s.lpr) + 255) / 256;
+  const int64_t zeros = std::min(kZeroGroups, (V + kZeroRows - 1) / kZeroRows);
+  const dim3 grid = grid_of(sums + zeros, 256, "embedding_grad", "elements");
+  hipLaunchKernelGGL((k_embed_sum<TW, TO, VEC>), grid, dim3(256), 0, stream, keys, pos, uint32_t(n), dy, dys, dw, part, V, D,
+                     scale, s, uint32_t(sums));
   if (s.pieces > 1)
-    hipLaunchKernelGGL((k_embed_join<TW, VEC>), dim3(uint32_t(s.pieces * s.chunks)), dim3(kJoinWaves * kWave), 0,
-                       stream, keys, uint32_t(n), part, dw, V, D, scale, s);
+    hipLaunchKernelGGL((k_embed_join<TW, VEC>), grid_of(s.pieces * s.chunks, kJoinWaves * kWave, "embedding_grad", "ids"),
+                       dim3(kJoinWaves * kWave), 0, stream, keys, uint32_t(n), part, dw, V, D, scale, s);
   RMM_HIP_CHECK(hipGetLastError());
 }
 

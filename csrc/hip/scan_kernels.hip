@@ -561,6 +561,7 @@ ScanPlan scan_plan(const ScanArgs& p, int type, int vec, const char* who) {
   const int64_t tiles = (chunks + s.units - 1) / s.units, cols = (p.D + (vec << s.lpr) - 1) / (vec << s.lpr);
   if (p.B > ((int64_t(1) << 31) - 1) / cols) throw std::invalid_argument(std::string(who) + ": too many sequences");
   s.chains = p.B * cols;
+  grid_of(s.chains, s.waves * kWave, who, "sequences");  // fewer than kEnoughChains where they are cut
   int64_t nseg = s.chains >= kEnoughChains ? 1 : std::min(tiles, kGroups / s.chains);
   s.per = int((tiles + nseg - 1) / nseg);
   s.nseg = int((tiles + s.per - 1) / s.per);
@@ -636,10 +637,10 @@ void gated_scan_step(const void* x, int64_t xs, const void* g, int64_t gs, const
                      float* out, void* y, int type, int64_t B, int64_t D, hipStream_t stream) {
   if (B <= 0 || D <= 0) return;
   const int64_t blocks = (B * D + 255) / 256;
-  if (blocks > (int64_t(1) << 31) - 1) throw std::invalid_argument("gated_scan_step: too many elements");
+  const dim3 grid = grid_of(blocks, 256, "gated_scan_step", "elements");
   dispatch_type(type, "gated_scan_step", [&](auto tag) {
     using T = decltype(tag);
-    hipLaunchKernelGGL((k_scan_step<T>), dim3(uint32_t(blocks)), dim3(256), 0, stream, static_cast<const T*>(x), xs,
+    hipLaunchKernelGGL((k_scan_step<T>), grid, dim3(256), 0, stream, static_cast<const T*>(x), xs,
                        static_cast<const T*>(g), gs, resets, h, out, static_cast<T*>(y), B, D);
   });
   RMM_HIP_CHECK(hipGetLastError());

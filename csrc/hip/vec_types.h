@@ -60,6 +60,12 @@ __device__ __forceinline__ void store_run(T* p, const float (&x)[N]) {
   *reinterpret_cast<RunOf<T, N>*>(p) = r;
 }
 
+// A grid of fewer than 2^32 threads, the most that HIP launches.
+inline dim3 grid_of(int64_t blocks, int threads, const char* who, const char* what) {
+  if (blocks > ((int64_t(1) << 32) - 1) / threads) throw std::invalid_argument(std::string(who) + ": too many " + what);
+  return dim3(uint32_t(blocks));
+}
+
 // Calls f(T{}) / f(A{}, B{}) for the element types of the codes.
 template <typename F>
 inline void dispatch_type(int t, const char* who, F&& f) {

@@ -141,7 +141,8 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: Union[int, torch.Tenso
 
     An element is dropped (zero, whatever it held) where its 16 random bits are below ``t = round(65536 p)``, else
     scaled by ``65536 / (65536 - t)``; the bits are those of Philox4x32-10 with key ``seed`` and counter
-    (index // 8, offset), so the CPU and the GPU draw the same mask. Elements are numbered in row-major order.
+    (index // 8, offset), so the CPU and the GPU draw the same mask. Elements are numbered in row-major order. (p above
+    1 - 2^-17 drops everything; the GPU takes fewer than 2^35 elements.)
 
     offset: the call's own number under the seed: an int, or an int64 tensor on x's device whose first element is read
     when the kernel runs (a graph replay then draws a new mask after each advance); the backward pass uses the value

@@ -216,6 +216,31 @@ def test_a_step_into_what_wants_gradients_is_refused(dev):
         ops.gated_scan_step(z, z, z, out=leaf)
 
 
+# ------------------------------------------------------------------------------------------ the ends of a launch
+@pytest.mark.gpu
+def test_sizes_that_pass_a_launch(cuda):
+    """A launch has fewer than 2^32 threads: lookups and gradients of larger sizes go round, scans say so."""
+    n = 1 << 26                                                       # 64 lanes a row
+    ids = torch.zeros(n, dtype=torch.int32, device=cuda)
+    ids[-1], ids[n // 2 - 1], ids[n // 2] = 1, 1, 2
+    w = torch.arange(3, device=cuda).half()[:, None].expand(3, 512).contiguous()
+    out = ops.embedding(ids, w)
+    assert out[-1].eq(1).all() and out[n // 2 - 1].eq(1).all() and out[n // 2].eq(2).all() and out[-2].eq(0).all()
+    assert float(out[:, 0].sum(dtype=torch.float64)) == 4 and float(out[:, -1].sum(dtype=torch.float64)) == 4
+    del out, ids
+    V = (1 << 30) + 77                                                # 64 rows to a group that writes zeros
+    w = torch.zeros(V, 1, dtype=torch.float16, device=cuda, requires_grad=True)
+    ids = torch.tensor([V - 1, 0, 1 << 29, V - 1, (1 << 28) + 5], device=cuda)
+    (dw,) = torch.autograd.grad(ops.embedding(ids, w), w, torch.ones(5, 1, dtype=torch.float16, device=cuda))
+    assert dw[ids, 0].tolist() == [2, 1, 1, 2, 1] and int((dw != 0).sum()) == 4
+    del w, dw
+    x = torch.zeros(1 << 26, 1, 1, dtype=torch.float16, device=cuda)
+    with pytest.raises(ValueError, match="too many sequences"):
+        ops.gated_scan(x, x)
+    y, h = ops.gated_scan(x[1:] + 1, x[1:])
+    assert (y == 0.5).all() and (h == 0.5).all()
+
+
 # ------------------------------------------------------------------------------------------ gates that are fully open
 @pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("L,D", [(40, 1), (40, 2), (300, 64), (700, 20), (2500, 130)])

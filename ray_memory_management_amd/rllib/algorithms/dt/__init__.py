@@ -139,8 +139,11 @@ class DT(Algorithm):
         obs_dim = int(np.prod(env.observation_space.shape))
         if c.seed is not None:
             torch.manual_seed(int(c.seed))
+        seed = 0
+        if c.counter_dropout:  # without a seed, masks of its own for each algorithm, as torch's dropout has
+            seed = int(torch.randint(1 << 62, ())) if c.seed is None else int(c.seed)
         self.model = DTModel(obs_dim, env.action_space.n, c.max_seq_len, self.horizon, c.embed_dim, c.num_layers,
-                             c.num_heads, c.embed_pdrop, c.attn_pdrop, c.counter_dropout, int(c.seed or 0)).to(self.device)
+                             c.num_heads, c.embed_pdrop, c.attn_pdrop, c.counter_dropout, seed).to(self.device)
         allobs = np.concatenate([e["obs"].reshape(len(e["obs"]), -1) for e in self.episodes]).astype(np.float64)
         self.model.obs_mean.copy_(torch.as_tensor(allobs.mean(0), dtype=torch.float32))
         self.model.obs_std.copy_(torch.as_tensor(allobs.std(0) + 1e-6, dtype=torch.float32))

@@ -133,6 +133,10 @@ class DT(Algorithm):
         self.episodes = episodes_from_batches(JsonReader(c.input_).read_all())
         if not self.episodes:
             raise ValueError("no complete episodes in the offline input")
+        n = env.action_space.n  # ops.embedding reads an id outside its table as zeros, so actions are looked at here
+        acts = np.concatenate([np.asarray(e["actions"]).reshape(-1) for e in self.episodes])
+        if acts.min() < 0 or acts.max() >= n:
+            raise ValueError(f"recorded actions are {acts.min()} to {acts.max()}, the environment has 0 to {n - 1}")
         self.horizon = int(c.horizon or max(len(e["dones"]) for e in self.episodes))
         dev = "cuda" if c.num_gpus and torch.cuda.is_available() else "cpu"
         self.device = torch.device(dev)
@@ -142,7 +146,7 @@ class DT(Algorithm):
         seed = 0
         if c.counter_dropout:  # without a seed, masks of its own for each algorithm, as torch's dropout has
             seed = int(torch.randint(1 << 62, ())) if c.seed is None else int(c.seed)
-        self.model = DTModel(obs_dim, env.action_space.n, c.max_seq_len, self.horizon, c.embed_dim, c.num_layers,
+        self.model = DTModel(obs_dim, n, c.max_seq_len, self.horizon, c.embed_dim, c.num_layers,
                              c.num_heads, c.embed_pdrop, c.attn_pdrop, c.counter_dropout, seed).to(self.device)
         allobs = np.concatenate([e["obs"].reshape(len(e["obs"]), -1) for e in self.episodes]).astype(np.float64)
         self.model.obs_mean.copy_(torch.as_tensor(allobs.mean(0), dtype=torch.float32))

@@ -1,4 +1,4 @@
-"""The Decision Transformer over recorded episodes: the seeds of its counter dropout."""
+"""The Decision Transformer over recorded episodes: the seeds of its counter dropout, actions outside the environment's."""
 import numpy as np
 import pytest
 
@@ -29,3 +29,10 @@ def test_counter_dropout_takes_a_seed_of_its_own(ray_shared, tmp_path):
         seeds.append(a.model.drop.seed)
         a.stop()
     assert seeds[2:] == [0, 5, 5] and len(set(seeds[:2])) == 2 and 0 not in seeds[:2]
+
+
+@pytest.mark.parametrize("actions", [[0, 1, 3], [0, -1, 1]])
+def test_recorded_actions_outside_the_environment_are_refused(ray_shared, tmp_path, actions):
+    _record(tmp_path, actions)
+    with pytest.raises(ValueError, match="recorded actions"):
+        _config(tmp_path).build()

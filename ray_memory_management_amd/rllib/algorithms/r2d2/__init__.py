@@ -251,6 +251,8 @@ class R2D2(DQN):
         super().validate_config(c)
         if c.burn_in >= c.replay_sequence_length:
             raise ValueError("burn_in must be shorter than replay_sequence_length")
+        if (c.model or {}).get("use_gated_scan"):
+            raise ValueError("R2D2's recurrent Q-model is an LSTM: use_gated_scan is not supported")
 
     def _setup_learner(self):
         c = self.algo_config

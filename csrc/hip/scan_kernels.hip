@@ -18,7 +18,8 @@
 // tile of chunks with the state behind this one, whose loads they issued before the exchange. With enough chains (one
 // sequence's 64 VEC channels) to fill the card, that reads x, g (and dy) once. With fewer, a chain is cut into segments:
 // k_scan_maps composes the map of each from a first reading, and the workgroups of the pass itself start from the maps
-// before theirs. Rows narrower than half a wave's reach put several chunks into a wave. VEC is 2 at any alignment.
+// before theirs. Rows narrower than half a wave's reach put several chunks into a wave. VEC is 2 at any alignment, 1 for a
+// single channel.
 //
 // Bound by memory, x, g, dy and the outputs crossing the bus once (twice for the inputs where chains are cut): bf16, us and
 // TB/s, forward / backward: [1024, 64, 1024] 78 (5.2) / 141 (4.8), [32, 2048, 1024] 89 (4.5) / 150 (4.5),
@@ -612,8 +613,7 @@ void gated_scan_fwd(const ScanArgs& p, const void* x, const void* g, void* y, in
     using T = decltype(tag);
     const int vec = p.D > 1 ? 2 : 1;
     const ScanPlan s = scan_plan(p, type, vec, "gated_scan");
-    const auto fwd = vec == 2 ? (s.lpr < 6 ? scan_fwd_t<T, 2, true> : scan_fwd_t<T, 2, false>)
-                              : (s.lpr < 6 ? scan_fwd_t<T, 1, true> : scan_fwd_t<T, 1, false>);
+    const auto fwd = vec == 1 ? scan_fwd_t<T, 1, true> : s.lpr < 6 ? scan_fwd_t<T, 2, true> : scan_fwd_t<T, 2, false>;
     fwd(p, s, static_cast<const T*>(x), static_cast<const T*>(g), static_cast<T*>(y), stream);
   });
 }
@@ -626,8 +626,7 @@ void gated_scan_bwd(const ScanArgs& p, const void* x, const void* g, const void*
     using T = decltype(tag);
     const int vec = p.D > 1 ? 2 : 1;
     const ScanPlan s = scan_plan(p, type, vec, "gated_scan backward");
-    const auto bwd = vec == 2 ? (s.lpr < 6 ? scan_bwd_t<T, 2, true> : scan_bwd_t<T, 2, false>)
-                              : (s.lpr < 6 ? scan_bwd_t<T, 1, true> : scan_bwd_t<T, 1, false>);
+    const auto bwd = vec == 1 ? scan_bwd_t<T, 1, true> : s.lpr < 6 ? scan_bwd_t<T, 2, true> : scan_bwd_t<T, 2, false>;
     bwd(p, s, static_cast<const T*>(x), static_cast<const T*>(g), static_cast<const T*>(dy), static_cast<T*>(dx),
         static_cast<T*>(dg), stream);
   });

@@ -39,17 +39,17 @@ def _same_device(who: str, ref: torch.Tensor, **tensors) -> None:
 
 # ------------------------------------------------------------------------------------------ embedding
 def _embedding_cpu(ids, weight, scale, padding_idx, dtype):
-    ids = ids.long()
-    ok = (ids >= 0) & (ids < weight.shape[0])
     w = weight if weight.dtype in (torch.float32, torch.float64) else weight.float()
     pad = padding_idx if padding_idx >= 0 else None
-    if bool(ok.all()):
-        out = nn.functional.embedding(ids, w, pad)
-    elif weight.shape[0] == 0:
-        out = w.new_zeros((*ids.shape, w.shape[1]))
+    if weight.shape[0] == 0:
+        out = w.sum() + w.new_zeros((*ids.shape, w.shape[1]))
     else:
-        out = nn.functional.embedding(torch.where(ok, ids, torch.zeros_like(ids)), w, pad)
-        out = torch.where(ok.unsqueeze(-1), out, torch.zeros((), dtype=out.dtype))
+        try:
+            out = nn.functional.embedding(ids, w, pad)
+        except (IndexError, RuntimeError):  # torch looks at each id on the CPU, and most calls have none outside
+            ok = (ids >= 0) & (ids < weight.shape[0])
+            out = nn.functional.embedding(torch.where(ok, ids, torch.zeros_like(ids)), w, pad)
+            out = torch.where(ok.unsqueeze(-1), out, torch.zeros((), dtype=out.dtype))
     return (out if scale == 1.0 else out * scale).to(dtype)
 
 

@@ -216,6 +216,18 @@ def test_a_step_into_what_wants_gradients_is_refused(dev):
         ops.gated_scan_step(z, z, z, out=leaf)
 
 
+# ------------------------------------------------------------------------------------------ empty tables
+@pytest.mark.parametrize("V,D", [(0, 4), (3, 0), (0, 0)])
+def test_embedding_of_an_empty_table(dev, V, D):
+    """Ids outside it, none at all, and the gradient, which is as empty."""
+    w = torch.zeros(V, D, device=dev, requires_grad=True)
+    for ids in (torch.tensor([0, 7, -3], device=dev), torch.empty(0, 2, dtype=torch.int32, device=dev)):
+        out = ops.embedding(ids, w, 2.0)
+        assert out.shape == (*ids.shape, D) and (out == 0).all()
+        (g,) = torch.autograd.grad(out.sum(), w)
+        assert g.shape == (V, D)
+
+
 # ------------------------------------------------------------------------------------------ the ends of a launch
 @pytest.mark.gpu
 def test_sizes_that_pass_a_launch(cuda):

@@ -8,8 +8,9 @@
 // (seed, offset). 16 bits an element keep the 20 wide multiplies of a counter below the time of its 8 elements'
 // memory traffic; the scale is that of the quantised rate, so the expectation of out is exactly x.
 //
-// Bound by memory: 32768 x 4097 fp16 87 us (6.2 TB/s), 8192 x 8192 bf16 with a residual 70 us (5.8), 4096 x 4096 fp32
-// 27 us (5.0). 8 elements a thread: one counter, and 16-byte loads of the 16-bit types.
+// Bound by memory: 32768 x 4097 fp16 88 us (6.1 TB/s), 8192 x 8192 bf16 with a residual 68 us (5.9), 4096 x 4096 fp32
+// 24 us (5.6, as the last-level cache holds part of it). 8 elements a thread: one counter, and 16-byte loads of the 16-bit
+// types.
 #include <hip/hip_runtime.h>
 
 #include <cmath>

@@ -3,14 +3,15 @@
 //   forward   out[i, :] = scale * W[id_i, :]; an id outside [0, V) gives a row of zeros
 //   gradient  dW[v, :]  = scale * sum over { i : id_i = v } of dy[i, :], all V rows written
 //
-// The sum over a token's rows is taken in fp32 in the order of the positions, so the result does not
-// depend on scheduling: the positions are sorted by id with a stable radix sort (no floating-point
-// atomics) and each row of dW is a walk over its segment of the sorted positions.
+// The sum over a token's rows is taken in fp32 and does not depend on scheduling: the positions are sorted by id with a
+// stable radix sort (no floating-point atomics) and cut into pieces, walked in order, whose sums are joined in a fixed
+// grouping. Sizes and types alone choose that grouping: the same call gives the same bits.
 //
-// All of it is bound by memory. 131071 tokens, 1536 columns, fp32 table of 100003 rows under bf16 rows: lookup 143 us
-// (402 MB written, 805 MB of rows read of which the caches serve the frequent ones), gradient 278 us = sort 30 + sums 238
-// (402 MB read, 614 MB written, 4.3 TB/s) + joins 10. 8192 tokens of 1024 bf16 columns, 32768 rows: lookup 7 us, gradient
-// 36 us = sort 18 (one workgroup: its latency) + sums 14 (5.9 TB/s) + joins 4.
+// All of it is bound by memory. 131071 tokens, 1536 columns, fp32 table of 100003 rows under bf16 rows: lookup 130 us
+// (402 MB written, 805 MB of rows read of which the caches serve the frequent ones), gradient 302 us = sort 30 + sums 266
+// (402 MB read, 614 MB written, 3.8 TB/s) + joins 6; on another card lookup 145, sums 238, joins 10. 8192 tokens of 1024
+// bf16 columns, 32768 rows: lookup 7 us, gradient 37 us = sort 18 (one workgroup: its latency) + sums 15 (5.6 TB/s) +
+// joins 4.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 

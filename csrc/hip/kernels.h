@@ -145,7 +145,7 @@ struct DenseFinalize {
 };
 
 // K22: embedding lookup out[i] = scale * W[id_i] (zeros for ids outside [0, V)) and its gradient
-// dW[v] = scale * sum of dy[i] over id_i = v, summed in fp32 in the order of i; `pad` (or -1) is a row whose
+// dW[v] = scale * sum of dy[i] over id_i = v, summed in fp32 in a fixed grouping; `pad` (or -1) is a row whose
 // gradient stays zero. W rows are wstride elements apart, dy rows dystride; out and dW are dense. Element types are
 // the codes of vec_types.h. The workspace holds embedding_grad_workspace(n, V, D) bytes, 16-byte aligned.
 void embedding_fwd(const void* ids, bool ids64, const void* w, int wtype, int64_t wstride, void* out, int otype,

@@ -22,10 +22,11 @@
 // single channel.
 //
 // Bound by memory, x, g, dy and the outputs crossing the bus once (twice for the inputs where chains are cut): bf16, us and
-// TB/s, forward / backward: [1024, 64, 1024] 78 (5.2) / 141 (4.8), [32, 2048, 1024] 89 (4.5) / 150 (4.5),
-// [16, 3001, 2048] 120 (4.9) / 214 (4.6), cut: [8, 2048, 1024] 35 / 49, [1, 65536, 1024] 128 / 195 of which the first
-// reading is 67 / 63 (4.0). About 20 instructions a step and channel, two of them at quarter rate, are half of the
-// arithmetic that these times leave room for; fp32 tensors have chunks of 8 steps to keep within the registers.
+// TB/s, forward / backward: [1024, 64, 1024] 80 (5.0) / 146 (4.6), [32, 2048, 1024] 87 (4.6) / 149 (4.5),
+// [16, 3001, 2048] 112 (5.3) / 203 (4.9), cut: [8, 2048, 1024] 35 / 48, [1, 65536, 1024] 130 / 190 of which the first
+// reading is 69 / 63 (4.0); fp32 [64, 1024, 512] 77 (5.2) / 139 (4.8). One step of 512 x 8192 bf16 13 us (4.4). About 20
+// instructions a step and channel, two of them at quarter rate, are half of the arithmetic that these times leave room for;
+// fp32 tensors have chunks of 8 steps to keep within the registers.
 //
 // A = 0 stands for a reset alone: what is before it is dropped, not multiplied by zero (it may be infinite or NaN).
 // Factors and products that underflow are held at the smallest denormal instead, so an infinite state stays infinite.

@@ -59,7 +59,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
 
     ids: int32 / int64 of any shape; an id outside ``[0, len(weight))`` gives a row of zeros and no gradient, so -1
     can mark padded places. weight: [V, D]. Its gradient is dense, ``scale * sum of dy over the places of an id``,
-    summed in fp32 in the order of the places (the same bits every time) and rounded once; the row ``padding_idx``
+    summed in fp32 in a grouping that the sizes and types alone choose (the same bits every time) and rounded once; the row ``padding_idx``
     (negative counts from the end) is read as any other and gets no gradient."""
     if ids.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"embedding: int32 or int64 ids, not {ids.dtype}")

@@ -253,20 +253,20 @@ def _held(v):
 
 
 class _Gate(torch.autograd.Function):
-    """The step's factor 1 - z of the state and its share z x of the input, z = sigmoid(g), with their relative precision on
-    both sides, in the gradient too (that of torch.sigmoid takes 1 - z by a subtraction, which has none left near z = 1)."""
+    """z = sigmoid(g) and the state's factor 1 - z with their relative precision on both sides, in the gradient too (that of
+    torch.sigmoid takes 1 - z by a subtraction, which has none left near z = 1)."""
 
     @staticmethod
-    def forward(ctx, g, x):
+    def forward(ctx, g):
         z, a = torch.sigmoid(g), torch.sigmoid(-g)
-        ctx.save_for_backward(z, a, x)
-        return _held(a), _held(z) * x
+        ctx.save_for_backward(z, a)
+        return z, _held(a)
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, da, du):
-        z, a, x = ctx.saved_tensors
-        return (du * x - da) * z * a, du * z
+    def backward(ctx, dz, da):
+        z, a = ctx.saved_tensors
+        return (dz - da) * z * a
 
 
 def _scan_cpu(x, gate, h0, resets, lengths):
@@ -278,7 +278,8 @@ def _scan_cpu(x, gate, h0, resets, lengths):
     if lengths is not None:
         live = (torch.arange(L) < lengths.unsqueeze(1)).unsqueeze(-1)
         x, gate = torch.where(live, x, zero), torch.where(live, gate, zero)
-    a, u = _Gate.apply(gate, x)
+    z, a = _Gate.apply(gate)
+    u = torch.where(z != 0, z * x, (_held(z) * x).detach())
     ys = []
     for t in range(L):
         prev = h if resets is None else torch.where((resets != 0)[:, t, None], torch.zeros((), dtype=st), h)

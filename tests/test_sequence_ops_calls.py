@@ -182,6 +182,20 @@ def test_a_capture_over_a_first_state_of_a_living_graph_is_refused(cuda, kind):
         assert (g == 0.125).all() and (h == 0.125).all() and g.dtype == h0.dtype
 
 
+def test_the_cpu_form_in_64_bits():
+    """Gradients against differences, and the gradient's own with respect to dy: dx is linear in it."""
+    x, g = (torch.randn(2, 5, 3, dtype=torch.float64, generator=torch.Generator().manual_seed(k)).requires_grad_()
+            for k in (0, 1))
+    h0 = torch.ones(2, 3, dtype=torch.float64, requires_grad=True)
+    assert torch.autograd.gradcheck(lambda *a: ops.gated_scan(*a), (x, g, h0))
+    y, _ = ops.gated_scan(x, g.detach())
+    dy = torch.ones_like(y, requires_grad=True)
+    (dx,) = torch.autograd.grad(y, x, dy, create_graph=True)
+    (ddy,) = torch.autograd.grad(dx, dy, torch.ones_like(dx))
+    ones, _ = ops.gated_scan(torch.ones_like(x), g.detach())
+    torch.testing.assert_close(ddy, ones, rtol=1e-12, atol=1e-12)  # the scan of ones: some 20 roundings of 2^-53
+
+
 # ------------------------------------------------------------------------------------------ a step's out
 def test_a_step_into_its_own_inputs(dev):
     """out over x, over the packed projection, over the gate, over the resets: as with an out of its own."""

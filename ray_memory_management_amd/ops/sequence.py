@@ -286,7 +286,7 @@ def _scan_cpu(x, gate, h0, resets, lengths):
         new = a[:, t] * prev + u[:, t]
         h = new if live is None else torch.where(live[:, t], new, h)
         ys.append(new if live is None else torch.where(live[:, t], new, torch.zeros((), dtype=new.dtype)))
-    return (torch.stack(ys, dim=1) if L else x.new_zeros((B, 0, D), dtype=st)), h
+    return (torch.stack(ys, dim=1), h) if L else (u.to(st), h + u.sum(dim=1))
 
 
 def _scan_parts(who, x, gate):

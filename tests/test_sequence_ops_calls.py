@@ -196,6 +196,16 @@ def test_the_cpu_form_in_64_bits():
     torch.testing.assert_close(ddy, ones, rtol=1e-12, atol=1e-12)  # the scan of ones: some 20 roundings of 2^-53
 
 
+def test_a_scan_of_no_steps_has_gradients(dev):
+    for gate in (torch.zeros(2, 0, 3, device=dev, requires_grad=True), None):
+        x = torch.zeros(2, 0, 3 if gate is not None else 6, device=dev, requires_grad=True)
+        y, h = ops.gated_scan(x, gate)
+        assert y.shape == (2, 0, 3) and (h == 0).all()
+        for v in torch.autograd.grad(y.sum() + h.sum(), (x,) if gate is None else (x, gate)):
+            assert v.shape[:2] == (2, 0)
+        assert h.requires_grad and y.requires_grad
+
+
 # ------------------------------------------------------------------------------------------ a step's out
 def test_a_step_into_its_own_inputs(dev):
     """out over x, over the packed projection, over the gate, over the resets: as with an out of its own."""
